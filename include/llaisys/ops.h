@@ -171,6 +171,59 @@ __C {
                                        llaisysTensor_t norm_weight, float eps,
                                        llaisysTensor_t weight, llaisysTensor_t weight_scale,
                                        llaisysTensor_t bias, uint8_t swiglu);
+    /* ---- KV cache in blocks, for many requests at once (no reference counterpart: its decoder
+     * keeps one contiguous cache per layer for one sequence, src/models/qwen2/attention.hpp:108-123).
+     * k_cache, v_cache [n_blocks, n_kvh, block, d] I8 and k_scale, v_scale [n_blocks, n_kvh] F32: a
+     * value is code * scale of its block and head.  block is a power of two in [16, 256], d a multiple
+     * of 16 up to 256.  block_table [requests, width] I32 holds each request's block ids in order; a
+     * token's slot is block id * block + offset.  What the device finds out of range is skipped and
+     * reported through llaisysTakeDeviceError (4); nothing outside the tensors is read or written. */
+
+    /* The tables of a step that takes request r from old_lens[r] to new_lens[r] cached tokens (I32;
+     * fewer: tokens taken back, 0: the request ended).  A request that grows takes the blocks it lacks
+     * from the ring of free blocks, one that shrinks gives back those it no longer needs (its
+     * table row keeps their ids): free_blocks [size] I32 holds ids at positions head .. tail - 1, modulo
+     * its size, and free_in = (head, tail) I64; free_out, the state after the step, may be free_in.  Blocks given back come
+     * behind the others, in the order of requests and blocks, and may be taken in the same step.
+     * row_starts [requests + 1] I32: the step's rows of request r are row_starts[r] ..
+     * row_starts[r + 1] - 1; slots and pos_ids [rows] I64: each row's slot and position (for
+     * llaisysROPEQK), -1 and 0 behind the last row.  A step that asks for more rows than slots holds,
+     * more blocks than are free, a length below 0 or beyond width * block, or with a state that is
+     * none, is refused as a whole: error 2, no rows, table, ring and state as they were. */
+    __export void llaisysPagedTables(llaisysTensor_t block_table, llaisysTensor_t slots,
+                                     llaisysTensor_t pos_ids, llaisysTensor_t row_starts,
+                                     llaisysTensor_t free_out, llaisysTensor_t old_lens,
+                                     llaisysTensor_t new_lens, llaisysTensor_t free_blocks,
+                                     llaisysTensor_t free_in, size_t block);
+    /* Rows k, v [rows, n_kvh, d] (F32 / BF16 / F16) quantized into their slots [rows] I64.  For each
+     * block and head, with A the largest |x| of its new rows (a NaN never raises it): the scale
+     * becomes s = max(scale, A / 127), or A / 127 where the rows begin at offset 0; codes before the rows
+     * become round(code * scale / s) where s grew; new codes are round(x / s), quotients rounded half to even as the exact
+     * ones, a NaN quotient 0.  The rows of a block must be consecutive rows of consecutive slots, as
+     * llaisysPagedTables makes them, else they are skipped (error 4); a block that two such runs of
+     * one call write holds undefined codes.  Rows of negative slot are skipped. */
+    __export void llaisysPagedKVAppendInt8(llaisysTensor_t k_cache, llaisysTensor_t k_scale,
+                                           llaisysTensor_t v_cache, llaisysTensor_t v_scale,
+                                           llaisysTensor_t k, llaisysTensor_t v,
+                                           llaisysTensor_t slots);
+    /* Rows k, v [rows, n_kvh, d] (F32 / BF16 / F16) = T(code * scale) of their slots [rows] I64 in any
+     * order, rounded to nearest (F16 too); rows of negative slot are left as they are. */
+    __export void llaisysPagedKVReadInt8(llaisysTensor_t k, llaisysTensor_t v, llaisysTensor_t k_cache,
+                                         llaisysTensor_t k_scale, llaisysTensor_t v_cache,
+                                         llaisysTensor_t v_scale, llaisysTensor_t slots);
+    /* Causal GQA attention of each request over its blocks: q, attn_val [rows, nh, d] of one float
+     * type, the rows of request r row_starts[r] .. row_starts[r + 1] - 1 and its kv_lens[r] (I32)
+     * cached tokens, these rows' own among them.  Row i of n sees tokens t <= kv_lens - n + i; f32
+     * softmax of (q . k) * scale; a row that sees nothing gives 0, a NaN score NaN.  Keys of a block id outside the pool
+     * are not attended (error 4); a request whose length or row starts are out of range is skipped
+     * (error 4).  Rows of no request are left as they are.  Outputs round to nearest (F16 too).  Any
+     * mix of prompts, chunks and single tokens goes in one call. */
+    __export void llaisysPagedAttentionInt8KV(llaisysTensor_t attn_val, llaisysTensor_t q,
+                                              llaisysTensor_t k_cache, llaisysTensor_t k_scale,
+                                              llaisysTensor_t v_cache, llaisysTensor_t v_scale,
+                                              llaisysTensor_t block_table,
+                                              llaisysTensor_t row_starts, llaisysTensor_t kv_lens,
+                                              float scale);
     /* Random sampling after argmax (no reference kernel: README.md:397-399 asks for a random
      * sample operator with temperature, top-k and top-p; python/llaisys/models/qwen2.py:216-218
      * takes the three and ignores them).  logits [V] or [rows, V] (F32 / BF16 / F16), out_idx

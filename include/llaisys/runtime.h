@@ -56,8 +56,10 @@ __C {
 
     /* Additive: errors found on the device cannot throw at launch time.  This waits for
      * the context stream of (device_type, device_id), returns the sticky device error
-     * code and clears it: 0 = none, 1 = an embedding id outside [0, vocab) (the reference
-     * throws "Embedding index out of bound", src/ops/embedding/cpu/embedding_cpu.cpp:18).
+     * code and clears it: 0 = none, else a sum of 1 = an embedding id outside [0, vocab) (the
+     * reference throws "Embedding index out of bound",
+     * src/ops/embedding/cpu/embedding_cpu.cpp:18), 2 = a step that llaisysPagedTables refused,
+     * 4 = a slot, block id, row start or length that an op of the paged KV cache skipped.
      * device_synchronize / stream_synchronize of the AMD table raise the same error
      * (print + throw, like every other LLAISYS error) when it is set. */
     __export int llaisysTakeDeviceError(llaisysDeviceType_t, int);

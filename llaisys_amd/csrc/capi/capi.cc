@@ -233,6 +233,37 @@ __C {
         llaisys::ops::randomSample(out_idx->tensor, logits->tensor, temperature, top_k, top_p, seed);
     }
 
+    void llaisysPagedTables(llaisysTensor_t block_table, llaisysTensor_t slots, llaisysTensor_t pos_ids,
+                            llaisysTensor_t row_starts, llaisysTensor_t free_out,
+                            llaisysTensor_t old_lens, llaisysTensor_t new_lens,
+                            llaisysTensor_t free_blocks, llaisysTensor_t free_in, size_t block) {
+        llaisys::ops::pagedTables(block_table->tensor, slots->tensor, pos_ids->tensor,
+                                  row_starts->tensor, free_out->tensor, old_lens->tensor,
+                                  new_lens->tensor, free_blocks->tensor, free_in->tensor, block);
+    }
+    void llaisysPagedKVAppendInt8(llaisysTensor_t k_cache, llaisysTensor_t k_scale,
+                                  llaisysTensor_t v_cache, llaisysTensor_t v_scale,
+                                  llaisysTensor_t k, llaisysTensor_t v, llaisysTensor_t slots) {
+        llaisys::ops::pagedKvAppendInt8(k_cache->tensor, k_scale->tensor, v_cache->tensor,
+                                        v_scale->tensor, k->tensor, v->tensor, slots->tensor);
+    }
+    void llaisysPagedKVReadInt8(llaisysTensor_t k, llaisysTensor_t v, llaisysTensor_t k_cache,
+                                llaisysTensor_t k_scale, llaisysTensor_t v_cache,
+                                llaisysTensor_t v_scale, llaisysTensor_t slots) {
+        llaisys::ops::pagedKvReadInt8(k->tensor, v->tensor, k_cache->tensor, k_scale->tensor,
+                                      v_cache->tensor, v_scale->tensor, slots->tensor);
+    }
+    void llaisysPagedAttentionInt8KV(llaisysTensor_t attn_val, llaisysTensor_t q,
+                                     llaisysTensor_t k_cache, llaisysTensor_t k_scale,
+                                     llaisysTensor_t v_cache, llaisysTensor_t v_scale,
+                                     llaisysTensor_t block_table, llaisysTensor_t row_starts,
+                                     llaisysTensor_t kv_lens, float scale) {
+        llaisys::ops::pagedAttentionInt8KV(attn_val->tensor, q->tensor, k_cache->tensor,
+                                           k_scale->tensor, v_cache->tensor, v_scale->tensor,
+                                           block_table->tensor, row_starts->tensor,
+                                           kv_lens->tensor, scale);
+    }
+
     // ---- model API: out of scope, exported so the reference ctypes loader binds --------
     struct LlaisysQwen2Model *llaisysQwen2ModelCreate(const struct LlaisysQwen2Meta *,
                                                       llaisysDeviceType_t, int *, int) {

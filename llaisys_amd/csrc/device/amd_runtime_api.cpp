@@ -191,7 +191,10 @@ int takeError(llaisysStream_t s) {
 
 void raiseIfError(llaisysStream_t s) {
     const int code = takeError(s);
-    if (code == 1) ASSERT(false, "Embedding index out of bound");
+    if (code & 1) ASSERT(false, "Embedding index out of bound");
+    ASSERT((code & kernels::kErrPagedTables) == 0,
+           "PagedTables: a length, the rows or the free blocks do not allow the step (nothing was changed)");
+    ASSERT((code & kernels::kErrPagedIndex) == 0, "Paged KV cache: a slot, block id, row start or length is out of range");
     if (code != 0) LLAISYS_FAIL(std::runtime_error, "device error code " << code, "device error");
 }
 

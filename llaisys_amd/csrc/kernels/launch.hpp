@@ -173,4 +173,54 @@ void randomSample(void *out_idx, bool i64, const void *logits, size_t rows, size
                   llaisysDataType_t dt, float temperature, int64_t top_k, float top_p,
                   uint64_t seed, void *ws, hipStream_t stream);
 
+// ---- KV cache in blocks (paged) ----------------------------------------------------------
+// codes [n_blocks, heads, block, dim] I8, scales [n_blocks, heads] F32; a slot is a token's
+// place, block id * block + offset.  `block` is a power of two in [16, 256], `dim` a multiple
+// of 16 up to 256, the code pools start on 16 bytes.
+struct PagedCache {
+    int8_t *k_codes, *v_codes;
+    float *k_scale, *v_scale;
+    size_t n_blocks, heads, block, dim;
+};
+// Bits of the device error word (0x1: embedding id).
+constexpr int kErrPagedTables = 0x2; // lengths, rows or free blocks that pagedTables refuses
+constexpr int kErrPagedIndex = 0x4;  // a slot, block id, row start or length that the cache's ops skip
+
+struct PagedTablesCall {
+    int32_t *table; // [requests, width]
+    int64_t *slots, *pos; // [rows]
+    int32_t *starts;      // [requests + 1]
+    int64_t *free_out;    // [2], may be free_in
+    const int32_t *old_lens, *new_lens; // [requests]
+    int32_t *ring; // [ring_size]
+    const int64_t *free_in;
+    size_t requests, width, rows, ring_size, block;
+    int *err;
+};
+// Scratch that pagedTables needs for these sizes.
+size_t pagedTablesWorkspaceBytes(const PagedTablesCall &c);
+void pagedTables(const PagedTablesCall &c, void *ws, hipStream_t stream);
+
+// Rows k, v [rows, heads, dim] quantized into the slots; a row of negative slot is skipped.
+void pagedKvAppendInt8(const PagedCache &c, const void *k, const void *v, const int64_t *slots,
+                       size_t rows, llaisysDataType_t dt, int *err, hipStream_t stream);
+
+// k, v [rows, heads, dim] = T(code * scale) of the slots; a row of negative slot is left as it is.
+void pagedKvReadInt8(void *k, void *v, const PagedCache &c, const int64_t *slots, size_t rows,
+                     llaisysDataType_t dt, int *err, hipStream_t stream);
+
+// Causal GQA attention of each request's rows of q [rows, nh, dim] over its cached tokens.
+struct PagedAttentionCall {
+    void *out;
+    const void *q;
+    PagedCache cache;
+    const int32_t *table; // [requests, width]
+    const int32_t *starts, *lens; // [requests + 1], [requests]
+    size_t rows, requests, width, nh;
+    float scale;
+    llaisysDataType_t dt;
+    int *err;
+};
+void pagedAttentionInt8KV(const PagedAttentionCall &c, hipStream_t stream);
+
 } // namespace llaisys::kernels

@@ -1,0 +1,254 @@
+// Writes and read-back of the KV cache in blocks: codes [n_blocks, heads, block, dim] I8 with one F32
+// scale for each (block, head).
+//
+// Append.  The rows of a step that go to one block are consecutive rows of consecutive slots.  With A the
+// largest |x| of those rows for a head, s0 the head's scale (0 where the rows begin at offset 0: the block
+// is new) and s = max(s0, A / 127), a new code is the whole number next to x / s, and where s grew the
+// codes before the rows become the whole numbers next to code * s0 / s.  A block's scale so only grows
+// while it fills; each growth rounds its older codes once more, by at most s / 2.
+//
+// Quotients are rounded as the exact quotient rounds (ties to even), so that one definition holds for any
+// way of computing it: with n = rint(x * (1 / s)), off by at most one, e = fma(-n, s, x) is exact, and n
+// moves by one where |e| > s / 2, or |e| = s / 2 with n odd.  (|n| < 2^8: n * s and x * 2^k / s agree in all but
+// the last bits, so e needs no more than 24 bits.)  Scales below 2^-96, where 1 / s or e may leave the
+// normal range, divide in f64, and so do the older codes.
+#include "common.hpp"
+#include "launch.hpp"
+#include "quantize.hpp"
+#include "rowplan.hpp"
+
+namespace llaisys::kernels {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+struct AppendArgs {
+    int8_t *codes[2];
+    float *scale[2];
+    const void *in[2];
+    const int64_t *slots;
+    int64_t rows, slot_end;
+    int heads, dim, shift, chunk;
+    int *err;
+};
+
+__device__ __forceinline__ float codeFast(float x, float s, float recip) {
+    float n = rintf(x * recip);
+    const float e = __builtin_fmaf(-n, s, x), h = 0.5f * s;
+    const bool odd = (int(n) & 1) != 0;
+    if (e > h || (e == h && odd)) n += 1.0f;
+    if (e < -h || (e == -h && odd)) n -= 1.0f;
+    return n;
+}
+
+__device__ __forceinline__ uint32_t codeExact(double x, double s) {
+    double n = rint(x / s);
+    if (n != n) return 0; // NaN quotient
+    n = n > 127.0 ? 127.0 : (n < -127.0 ? -127.0 : n);
+    return uint32_t(int32_t(n)) & 0xFFu;
+}
+
+// Codes of one 16-byte vector; s is the block's scale, fast where the f32 rule holds.
+template <typename T>
+__device__ __forceinline__ void storeVec(int8_t *to, const v4u &r, float s, float recip, bool fast) {
+    constexpr int N = Fmt<T>::kVec;
+    float f[N];
+    Fmt<T>::unpack(r, f);
+    uint32_t c[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        if (fast) {
+            const float n = codeFast(f[e], s, recip);
+            c[e] = n == n ? uint32_t(int32_t(n)) & 0xFFu : 0u;
+        } else {
+            c[e] = codeExact(f[e], s);
+        }
+    }
+    uint32_t w[N / 4];
+#pragma unroll
+    for (int e = 0; e < N / 4; ++e) w[e] = packCodes4(c + 4 * e);
+    __builtin_memcpy(__builtin_assume_aligned(to, N), w, N);
+}
+
+// A block of threads takes `chunk` rows of one head of k or v, and of them the rows where a cache block begins.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void pagedAppend(AppendArgs a) {
+    constexpr int N = Fmt<T>::kVec;
+    constexpr int kKeep = 8; // vectors a thread keeps between the maximum and the codes
+    __shared__ float red[kThreads / kWave];
+    __shared__ int run_end;
+    const int head = blockIdx.y, kv = blockIdx.z;
+    const int nv = a.dim / N, block = 1 << a.shift;
+    const int64_t t_end = min(a.rows, (int64_t(blockIdx.x) + 1) * a.chunk);
+    for (int64_t t = int64_t(blockIdx.x) * a.chunk; t < t_end; ++t) {
+        const int64_t slot = a.slots[t];
+        if (slot < 0) continue;
+        if (slot >= a.slot_end) {
+            if (threadIdx.x == 0) atomicOr(a.err, kErrPagedIndex);
+            continue;
+        }
+        const int64_t id = slot >> a.shift;
+        if (t > 0 && a.slots[t - 1] >= 0 && (a.slots[t - 1] >> a.shift) == id) continue; // not the block's first row
+        // the run of rows of this block; rows that do not follow each other are refused
+        __syncthreads();
+        if (threadIdx.x == 0) run_end = block + 1;
+        __syncthreads();
+        bool follows = true;
+        for (int i = threadIdx.x; i <= block; i += kThreads) {
+            const int64_t st = t + i < a.rows ? a.slots[t + i] : -1;
+            if (st < 0 || (st >> a.shift) != id)
+                atomicMin(&run_end, i);
+        }
+        __syncthreads();
+        const int run = run_end;
+        for (int i = threadIdx.x; i < run; i += kThreads) follows = follows && a.slots[t + i] == slot + i;
+        if (!__syncthreads_and(follows)) {
+            if (threadIdx.x == 0) atomicOr(a.err, kErrPagedIndex);
+            continue;
+        }
+        const int first = int(slot & (block - 1)), n = run * nv;
+        const char *in = static_cast<const char *>(a.in[kv]);
+        const auto at = [&](int j) {
+            const int row = j / nv;
+            return (size_t(t + row) * a.heads + head) * a.dim + size_t(j - row * nv) * N;
+        };
+        v4u keep[kKeep];
+        float amax = 0.0f;
+        const auto fold = [&](const v4u &r) {
+            float f[N];
+            Fmt<T>::unpack(r, f);
+#pragma unroll
+            for (int e = 0; e < N; ++e) amax = MaxOp::apply(amax, fabsf(f[e]));
+        };
+#pragma unroll
+        for (int i = 0; i < kKeep; ++i) {
+            const int j = threadIdx.x + i * kThreads;
+            keep[i] = j < n ? load16<T>(in, at(j)) : v4u{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int i = 0; i < kKeep; ++i) fold(keep[i]);
+        for (int j = threadIdx.x + kKeep * kThreads; j < n; j += kThreads) fold(load16<T>(in, at(j)));
+        const size_t tile = size_t(id) * a.heads + head;
+        const float s0 = first ? a.scale[kv][tile] : 0.0f;
+        amax = groupReduce<kThreads, MaxOp>(amax, red);
+        const float grown = amax / 127.0f, s = grown > s0 ? grown : s0;
+        int8_t *codes = a.codes[kv] + (tile << a.shift) * a.dim;
+        if (threadIdx.x == 0 && (s != s0 || first == 0)) a.scale[kv][tile] = s;
+        if (first && s != s0) {
+            for (int j = threadIdx.x; j < first * (a.dim / 16); j += kThreads) {
+                v4u r = *reinterpret_cast<const v4u *>(codes + j * 16);
+                uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t c[4];
+#pragma unroll
+                    for (int b = 0; b < 4; ++b)
+                        c[b] = codeExact(double(int32_t(w[e] << (24 - 8 * b)) >> 24) * double(s0), double(s));
+                    w[e] = packCodes4(c);
+                }
+                *reinterpret_cast<v4u *>(codes + j * 16) = v4u{w[0], w[1], w[2], w[3]};
+            }
+        }
+        const float recip = 1.0f / s;
+        const bool fast = s >= 0x1p-96f && s <= 0x1p120f;
+#pragma unroll
+        for (int i = 0; i < kKeep; ++i) {
+            const int j = threadIdx.x + i * kThreads;
+            if (j < n) storeVec<T>(codes + first * a.dim + j * N, keep[i], s, recip, fast);
+        }
+        for (int j = threadIdx.x + kKeep * kThreads; j < n; j += kThreads)
+            storeVec<T>(codes + first * a.dim + j * N, load16<T>(in, at(j)), s, recip, fast);
+    }
+}
+
+struct ReadArgs {
+    void *out[2];
+    const int8_t *codes[2];
+    const float *scale[2];
+    const int64_t *slots;
+    int64_t n, slot_end; // 8-code vectors of k or v
+    DivU64 per_row, per_head;
+    int heads, dim, shift;
+    int *err;
+};
+
+// f16 rounds to nearest even (the conversion instruction), bf16 likewise, f32 is the product.
+template <typename T>
+__device__ __forceinline__ void storeRounded(void *out, size_t elem, const float *f) {
+    if constexpr (Fmt<T>::kVec == 4) {
+        store16Stream<T>(out, elem, Fmt<T>::pack(f));
+        store16Stream<T>(out, elem + 4, Fmt<T>::pack(f + 4));
+    } else if constexpr (std::is_same_v<T, F16>) {
+        typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+        v8h h;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = _Float16(f[e]);
+        store16Stream<T>(out, elem, __builtin_bit_cast(v4u, h));
+    } else {
+        store16Stream<T>(out, elem, Fmt<T>::packQ(f));
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void pagedRead(ReadArgs a) {
+    const int kv = blockIdx.y;
+    for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < a.n; i += int64_t(gridDim.x) * kThreads) {
+        const int64_t t = int64_t(a.per_row.div(uint64_t(i)));
+        const int in_row = int(i - t * (int64_t(a.heads) * (a.dim / 8)));
+        const int64_t slot = a.slots[t];
+        if (slot < 0) continue;
+        if (slot >= a.slot_end) {
+            atomicOr(a.err, kErrPagedIndex);
+            continue;
+        }
+        const int head = int(a.per_head.div(uint64_t(in_row))), c = (in_row - head * (a.dim / 8)) * 8;
+        const int64_t tile = (slot >> a.shift) * a.heads + head;
+        const int8_t *from = a.codes[kv] + ((tile << a.shift) + (slot & ((1 << a.shift) - 1))) * a.dim + c;
+        uint32_t w[2];
+        __builtin_memcpy(w, __builtin_assume_aligned(from, 8), 8);
+        const float s = a.scale[kv][tile];
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = float(int32_t(w[e / 4] << (24 - 8 * (e % 4))) >> 24) * s;
+        storeRounded<T>(a.out[kv], size_t(i) * 8, f);
+    }
+}
+
+} // namespace
+
+void pagedKvAppendInt8(const PagedCache &c, const void *k, const void *v, const int64_t *slots, size_t rows,
+                       llaisysDataType_t dt, int *err, hipStream_t s) {
+    if (rows == 0 || c.heads == 0 || c.dim == 0) return;
+    // Few rows: a block of threads each, so that a step of one token per request runs in one round.
+    // Many: 16 rows a block (a cache block has 16 rows or more, so that prompts find one or two beginnings there).
+    const int chunk = rows * c.heads * 2 <= 16384 ? 1 : 16;
+    const AppendArgs a{{c.k_codes, c.v_codes}, {c.k_scale, c.v_scale}, {k, v}, slots, int64_t(rows),
+                       int64_t(c.n_blocks * c.block), int(c.heads), int(c.dim), __builtin_ctzll(c.block), chunk, err};
+    const dim3 grid(unsigned((rows + chunk - 1) / chunk), unsigned(c.heads), 2);
+    switch (dt) {
+    case LLAISYS_DTYPE_F32: pagedAppend<F32><<<grid, kThreads, 0, s>>>(a); return;
+    case LLAISYS_DTYPE_BF16: pagedAppend<BF16><<<grid, kThreads, 0, s>>>(a); return;
+    case LLAISYS_DTYPE_F16: pagedAppend<F16><<<grid, kThreads, 0, s>>>(a); return;
+    default: return;
+    }
+}
+
+void pagedKvReadInt8(void *k, void *v, const PagedCache &c, const int64_t *slots, size_t rows, llaisysDataType_t dt,
+                     int *err, hipStream_t s) {
+    const size_t per_row = c.heads * (c.dim / 8), n = rows * per_row;
+    if (n == 0) return;
+    const ReadArgs a{{k, v}, {c.k_codes, c.v_codes}, {c.k_scale, c.v_scale}, slots, int64_t(n),
+                     int64_t(c.n_blocks * c.block), DivU64(per_row), DivU64(c.dim / 8), int(c.heads), int(c.dim),
+                     __builtin_ctzll(c.block), err};
+    const size_t blocks = (n + kThreads - 1) / kThreads;
+    const dim3 grid(unsigned(blocks < (size_t(1) << 24) ? blocks : (size_t(1) << 24)), 2);
+    switch (dt) {
+    case LLAISYS_DTYPE_F32: pagedRead<F32><<<grid, kThreads, 0, s>>>(a); return;
+    case LLAISYS_DTYPE_BF16: pagedRead<BF16><<<grid, kThreads, 0, s>>>(a); return;
+    case LLAISYS_DTYPE_F16: pagedRead<F16><<<grid, kThreads, 0, s>>>(a); return;
+    default: return;
+    }
+}
+
+} // namespace llaisys::kernels

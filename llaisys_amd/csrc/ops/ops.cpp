@@ -7,35 +7,11 @@
 // output would be an out-of-bounds write, not a CPU heap overrun.  Only the AMD device
 // computes; CPU tensors raise "Unsupported device" (the reference CPU kernels are the
 // test oracle, not a fallback of this library).
-#include "ops.hpp"
-
-#include "../device/runtime_api.hpp"
-#include "../kernels/launch.hpp"
-#include "../utils/check.hpp"
-#include "../utils/types.hpp"
+#include "op_common.hpp"
 
 namespace llaisys::ops {
 
 namespace {
-
-bool isFloat(llaisysDataType_t dt) {
-    return dt == LLAISYS_DTYPE_F32 || dt == LLAISYS_DTYPE_BF16 || dt == LLAISYS_DTYPE_F16;
-}
-
-void requireFloat(llaisysDataType_t dt) {
-    if (!isFloat(dt)) EXCEPTION_UNSUPPORTED_DATATYPE(dt);
-}
-
-// Makes the device of `t` current and returns its stream; only the AMD device computes.
-hipStream_t streamFor(const tensor_t &t) {
-    if (t->deviceType() != LLAISYS_DEVICE_AMD) EXCEPTION_UNSUPPORTED_DEVICE;
-    auto &ctx = core::context();
-    ctx.setDevice(t->deviceType(), t->deviceId());
-    return static_cast<hipStream_t>(ctx.runtime().stream());
-}
-
-// Reports a failed launch (bad configuration, no code object for this GPU) at the call.
-void launched(const char *op) { device::amd::check(hipGetLastError(), op); }
 
 size_t lastDim(const tensor_t &t) {
     ASSERT(t->ndim() >= 1, "tensor must have at least one dimension");
@@ -569,14 +545,6 @@ void linearW8A16(tensor_t out, tensor_t in, tensor_t w_codes, tensor_t w_scale, 
               in->deviceId(), s);
     launched("linearW8A16");
 }
-
-namespace {
-// Byte ranges of two contiguous tensors intersect.
-bool overlaps(const tensor_t &a, const tensor_t &b) {
-    const std::byte *a0 = a->data(), *b0 = b->data();
-    return a0 < b0 + b->numel() * b->elementSize() && b0 < a0 + a->numel() * a->elementSize();
-}
-} // namespace
 
 // rms_norm (after an optional residual add) fused ahead of a linear, and optionally swiglu
 // after it: the decoder's input_layernorm -> q/k/v projections and add ->

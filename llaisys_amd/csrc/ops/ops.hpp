@@ -40,5 +40,15 @@ void rmsNormLinear(tensor_t out, tensor_t residual_out, tensor_t in, tensor_t re
 void ropeKvAppendInt8(tensor_t q_out, tensor_t q_in, tensor_t k_in, tensor_t v_in,
                       tensor_t pos_ids, float theta, tensor_t k_cache, tensor_t k_scale,
                       tensor_t v_cache, tensor_t v_scale, size_t pos);
+void pagedTables(tensor_t block_table, tensor_t slots, tensor_t pos_ids, tensor_t row_starts,
+                 tensor_t free_out, tensor_t old_lens, tensor_t new_lens, tensor_t free_blocks,
+                 tensor_t free_in, size_t block);
+void pagedKvAppendInt8(tensor_t k_cache, tensor_t k_scale, tensor_t v_cache, tensor_t v_scale,
+                       tensor_t k, tensor_t v, tensor_t slots);
+void pagedKvReadInt8(tensor_t k, tensor_t v, tensor_t k_cache, tensor_t k_scale, tensor_t v_cache,
+                     tensor_t v_scale, tensor_t slots);
+void pagedAttentionInt8KV(tensor_t attn_val, tensor_t q, tensor_t k_cache, tensor_t k_scale,
+                          tensor_t v_cache, tensor_t v_scale, tensor_t block_table,
+                          tensor_t row_starts, tensor_t kv_lens, float scale);
 
 } // namespace llaisys::ops

@@ -38,6 +38,10 @@ ADDED_OPS = {
     "llaisysLinearW8A16": [T, T, T, T, T],
     "llaisysRandomSample": [T, T, c_float, c_int64, c_float, c_uint64],
     "llaisysRmsNormLinear": [T, T, T, T, T, c_float, T, T, T, c_uint8],
+    "llaisysPagedTables": [T, T, T, T, T, T, T, T, T, c_size_t],
+    "llaisysPagedKVAppendInt8": [T, T, T, T, T, T, T],
+    "llaisysPagedKVReadInt8": [T, T, T, T, T, T, T],
+    "llaisysPagedAttentionInt8KV": [T, T, T, T, T, T, T, T, T, c_float],
 }
 
 

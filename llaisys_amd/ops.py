@@ -153,3 +153,46 @@ class Ops:
                       seed: int):
         LIB_LLAISYS.llaisysRandomSample(out_idx.lib_tensor(), logits.lib_tensor(), c_float(temperature),
                                         c_int64(top_k), c_float(top_p), c_uint64(seed & (2 ** 64 - 1)))
+
+    # ---- KV cache in blocks, for many requests at once ---------------------------------
+    @staticmethod
+    def paged_tables(block_table: Tensor, slots: Tensor, pos_ids: Tensor, row_starts: Tensor,
+                     free_out: Tensor, old_lens: Tensor, new_lens: Tensor, free_blocks: Tensor,
+                     free_in: Tensor, block: int):
+        """Tables of a step that takes each request from old_lens to new_lens tokens
+        (llaisysPagedTables): blocks taken from or given back to the ring, and the slot and
+        position of each new row."""
+        LIB_LLAISYS.llaisysPagedTables(block_table.lib_tensor(), slots.lib_tensor(),
+                                       pos_ids.lib_tensor(), row_starts.lib_tensor(),
+                                       free_out.lib_tensor(), old_lens.lib_tensor(),
+                                       new_lens.lib_tensor(), free_blocks.lib_tensor(),
+                                       free_in.lib_tensor(), c_size_t(block))
+
+    @staticmethod
+    def paged_kv_append_int8(k_cache: Tensor, k_scale: Tensor, v_cache: Tensor, v_scale: Tensor,
+                             k: Tensor, v: Tensor, slots: Tensor):
+        """k and v rows quantized into their slots, a scale per block and head
+        (llaisysPagedKVAppendInt8)."""
+        LIB_LLAISYS.llaisysPagedKVAppendInt8(k_cache.lib_tensor(), k_scale.lib_tensor(),
+                                             v_cache.lib_tensor(), v_scale.lib_tensor(),
+                                             k.lib_tensor(), v.lib_tensor(), slots.lib_tensor())
+
+    @staticmethod
+    def paged_kv_read_int8(k: Tensor, v: Tensor, k_cache: Tensor, k_scale: Tensor, v_cache: Tensor,
+                           v_scale: Tensor, slots: Tensor):
+        """k and v rows of the slots, dequantized (llaisysPagedKVReadInt8)."""
+        LIB_LLAISYS.llaisysPagedKVReadInt8(k.lib_tensor(), v.lib_tensor(), k_cache.lib_tensor(),
+                                           k_scale.lib_tensor(), v_cache.lib_tensor(),
+                                           v_scale.lib_tensor(), slots.lib_tensor())
+
+    @staticmethod
+    def paged_attention_int8kv(attn_val: Tensor, q: Tensor, k_cache: Tensor, k_scale: Tensor,
+                               v_cache: Tensor, v_scale: Tensor, block_table: Tensor,
+                               row_starts: Tensor, kv_lens: Tensor, scale: float):
+        """Causal attention of each request's rows over its cached tokens
+        (llaisysPagedAttentionInt8KV)."""
+        LIB_LLAISYS.llaisysPagedAttentionInt8KV(attn_val.lib_tensor(), q.lib_tensor(),
+                                                k_cache.lib_tensor(), k_scale.lib_tensor(),
+                                                v_cache.lib_tensor(), v_scale.lib_tensor(),
+                                                block_table.lib_tensor(), row_starts.lib_tensor(),
+                                                kv_lens.lib_tensor(), c_float(scale))
