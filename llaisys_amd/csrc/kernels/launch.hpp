@@ -64,13 +64,15 @@ void argmaxRows(void *idx, bool idx_i64, void *val, const void *vals, size_t row
 
 // Library scratch layout (zeroed once when allocated): bytes [0, 256) hold the flat argmax's
 // completion counter and key (16 of them, one per row of a few-row argmax) and [kSampleStateOffset, kScratchReserved) the sampler's per-row
-// histograms and counters; both stay zero between launches.  Other users of the scratch
-// start at kScratchReserved.
+// histograms and counters; behind it the arrival counters of the attention over the paged
+// cache.  All stay zero between launches.  Other users of the scratch start at kScratchReserved.
 constexpr size_t kSampleRows = 16;            // rows per sampler launch
 constexpr size_t kSampleRowStateBytes = 16400;
 constexpr size_t kSampleStateOffset = 256;
-constexpr size_t kScratchReserved =
+constexpr size_t kPagedCounters = 4096;       // of each of two levels
+constexpr size_t kPagedCountersOffset =
     (kSampleStateOffset + kSampleRows * kSampleRowStateBytes + 255) / 256 * 256;
+constexpr size_t kScratchReserved = kPagedCountersOffset + 2 * kPagedCounters * sizeof(unsigned);
 
 // Flat argmax over n elements; `workspace` (>= argmaxWorkspaceBytes(n)) holds the
 // completion counter (first kScratchReserved bytes, zero before the first call; the kernel
@@ -221,6 +223,9 @@ struct PagedAttentionCall {
     llaisysDataType_t dt;
     int *err;
 };
-void pagedAttentionInt8KV(const PagedAttentionCall &c, hipStream_t stream);
+// Bytes behind the reserved head of the scratch that let the call split its keys.
+size_t pagedAttentionWorkspaceBytes(const PagedAttentionCall &c);
+// `ws`: the library scratch (reserved head and `ws_bytes` behind it), or null: no tile's keys are split.
+void pagedAttentionInt8KV(const PagedAttentionCall &c, void *ws, size_t ws_bytes, hipStream_t stream);
 
 } // namespace llaisys::kernels

@@ -1,0 +1,331 @@
+// Shared by the kernels of the attention over the KV cache in blocks (paged_attention*.hip).
+//
+// The rows of a request and a kv head are its n tokens times the group = nh / heads q heads that share the
+// kv head: row m is token m / group, head m % group of the group.  A tile of rows attends its keys in steps
+// of 64; where the tiles of all requests would leave compute units idle, the keys are split into chunks of a
+// whole number of steps, and whoever finishes a tile's last chunk merges them.
+//
+// Codes meet the matrix instructions as f16: a code is a whole number of magnitude <= 127, exact in f16, for
+// every element type of q.  Rows of q are multiplied by a power of two that brings their largest element to
+// [2^14, 2^15): bf16 and f16 rows then are exact f16 (but for elements below 2^-38 of the row's largest), f32 rows
+// enter as two f16 parts (22 bits).  Weights p = 2^(t - m) lie in [0, 1], enter times 2^15 (f16's normal range
+// then goes down to 2^-29), and in two parts where the rows are f16 or f32; bf16 rows round the result to 8 bits, 11 for
+// a weight are enough.  A block's scale of v multiplies the weights as its ratio to the largest seen so
+// far, so that nothing leaves f16's range.
+#pragma once
+
+#include "common.hpp"
+#include "launch.hpp"
+
+namespace llaisys::kernels {
+
+constexpr int kStep = 64;    // keys of a step
+constexpr int kFan = 16;     // chunks merged at once
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kCodeUnit = 0x1p-9f; // a code's f16 value is code * kCodeUnit
+constexpr float kWeightBits = 15.0f; // weights are 2^(t - m + kWeightBits)
+
+struct PagedAttnArgs {
+    void *out;
+    const void *q;
+    const int8_t *k_codes, *v_codes;
+    const float *k_scale, *v_scale;
+    const int32_t *table, *starts, *lens;
+    float *part;        // [2][splits] partials: of chunks, of groups of chunks
+    unsigned *arrived;  // [2][kPagedCounters], 0 between launches
+    unsigned splits;
+    unsigned target;    // chunks wanted over all requests and heads; 0: no tile is split
+    int64_t rows, requests, width, n_blocks;
+    int nh, heads, group, dim, shift;
+    float scale;
+    int *err;
+};
+
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+
+// Two codes, given as code + 128 in bytes 0 and 2 of a word, as f16: the bytes are f16 subnormals of 2^-24,
+// and one packed fma brings them to code * 2^-9, exactly.
+__device__ __forceinline__ v2h codePair(uint32_t bytes) {
+    const v2h up{_Float16(0x1p15f), _Float16(0x1p15f)}, bias{_Float16(-0.25f), _Float16(-0.25f)};
+    return __builtin_elementwise_fma(__builtin_bit_cast(v2h, bytes), up, bias);
+}
+
+struct Pairs {
+    v2h p[4];
+};
+__device__ __forceinline__ v8h join(const Pairs &x) { return __builtin_bit_cast(v8h, x); }
+
+// Eight codes in a row (two words) as f16.
+__device__ __forceinline__ v8h codes8(uint32_t lo, uint32_t hi) {
+    lo ^= 0x80808080u;
+    hi ^= 0x80808080u;
+    return join(Pairs{{codePair(__builtin_amdgcn_perm(lo, lo, 0x0c010c00u)), codePair(__builtin_amdgcn_perm(lo, lo, 0x0c030c02u)),
+                       codePair(__builtin_amdgcn_perm(hi, hi, 0x0c010c00u)), codePair(__builtin_amdgcn_perm(hi, hi, 0x0c030c02u))}});
+}
+
+// f32 -> f16, to nearest; what it leaves over, again in f16.
+__device__ __forceinline__ v8h narrow8(const float *f) {
+    v8h h;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = _Float16(f[e]);
+    return h;
+}
+__device__ __forceinline__ v8h rest8(const float *f, const v8h &h) {
+    v8h l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) l[e] = _Float16(f[e] - float(h[e]));
+    return l;
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const void *base, size_t elem, float *f) {
+    Fmt<T>::unpack(load16<T>(base, elem), f);
+    if constexpr (Fmt<T>::kVec == 4) Fmt<T>::unpack(load16<T>(base, elem + 4), f + 4);
+}
+
+// Eight outputs, rounded once, to nearest (f16 by the conversion instruction).
+template <typename T>
+__device__ __forceinline__ void store8(void *base, size_t elem, const float *f) {
+    if constexpr (Fmt<T>::kVec == 4) {
+        store16<T>(base, elem, Fmt<T>::pack(f));
+        store16<T>(base, elem + 4, Fmt<T>::pack(f + 4));
+    } else if constexpr (std::is_same_v<T, F16>) {
+        store16<T>(base, elem, __builtin_bit_cast(v4u, narrow8(f)));
+    } else {
+        store16<T>(base, elem, Fmt<T>::packQ(f));
+    }
+}
+
+// Largest finite magnitude of f's elements so far.
+__device__ __forceinline__ float foldFinite(float m, const float *f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float x = fabsf(f[e]);
+        m = x < INFINITY && x > m ? x : m;
+    }
+    return m;
+}
+// Exponent that brings `top` to [2^14, 2^15).
+__device__ __forceinline__ int rowExponent(float top) { return top > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0; }
+
+// What a block of threads works at: a tile of one request's rows and a chunk of its keys.
+struct Item {
+    bool any;
+    int64_t start;     // first row of the request in q
+    int64_t request;
+    int n, len;        // rows and cached tokens of the request
+    int tile;
+    int step0, step1;  // steps of the chunk (not cut to what the tile sees)
+    int chunk, chunks; // of the tile
+    unsigned split;    // partial of the tile's first chunk, where chunks > 1
+};
+
+// The item of index `index`: requests in order, of each its tiles, of each its chunks.  Every wave finds it by
+// itself: sums over the requests 64 at a time, so that no table of items has to be made before.
+template <int kTile>
+__device__ Item findItem(const PagedAttnArgs &a, unsigned index, int per_chunk, bool report) {
+    const int lane = threadIdx.x % kWave;
+    const auto request = [&](int64_t r, int &start, int &n, int &len) { // false: out of range, skipped
+        start = n = len = 0;
+        if (r >= a.requests) return true;
+        const int64_t s0 = a.starts[r], s1 = a.starts[r + 1], k = a.lens[r];
+        if (s0 < 0 || s1 < s0 || s1 > a.rows || k < 0 || k > (a.width << a.shift)) return false;
+        start = int(s0);
+        n = int(s1 - s0);
+        len = int(k);
+        return true;
+    };
+    const auto tilesOf = [&](int n) { return unsigned((int64_t(n) * a.group + kTile - 1) / kTile); };
+    const auto stepsOf = [&](int len) { return unsigned((int64_t(len) + kStep - 1) / kStep); };
+    // steps of a chunk
+    unsigned per = 0x7FFFFFFFu;
+    int start, n, len;
+    if (a.target || report) {
+        uint64_t total = 0;
+        bool fine = true;
+        for (int64_t r0 = 0; r0 < a.requests; r0 += kWave) {
+            fine = request(r0 + lane, start, n, len) && fine;
+            total += uint64_t(tilesOf(n)) * stepsOf(len);
+        }
+#pragma unroll
+        for (int m = 1; m < kWave; m <<= 1) total += (uint64_t(uint32_t(__shfl_xor(int(total >> 32), m, kWave))) << 32) | uint32_t(__shfl_xor(int(uint32_t(total)), m, kWave));
+        fine = !__any(!fine);
+        if (report && !fine && lane == 0) atomicOr(a.err, kErrPagedIndex);
+        // row starts that go back may make more items than the grid has: a tile whose chunks did not all run
+        // would leave its counter behind, so nothing is split then
+        if (a.target && fine) {
+            const uint64_t want = (total * unsigned(a.heads) + a.target - 1) / a.target;
+            const uint64_t up = (want + per_chunk - 1) / per_chunk * per_chunk;
+            per = up < per_chunk ? unsigned(per_chunk) : (up < per ? unsigned(up) : per);
+        }
+    }
+    unsigned items = 0, splits = 0; // before this group of requests
+    for (int64_t r0 = 0; r0 < a.requests; r0 += kWave) {
+        request(r0 + lane, start, n, len);
+        const unsigned tiles = tilesOf(n), steps = stepsOf(len), chunks = steps > per ? (steps + per - 1) / per : 1;
+        unsigned mine = tiles * chunks, split = chunks > 1 ? mine : 0, to = mine, sto = split;
+#pragma unroll
+        for (int d = 1; d < kWave; d <<= 1) {
+            const unsigned u = __shfl_up(to, d, kWave), v = __shfl_up(sto, d, kWave);
+            to += lane >= d ? u : 0;
+            sto += lane >= d ? v : 0;
+        }
+        const uint64_t hit = __ballot(index >= items + to - mine && index < items + to);
+        if (hit) {
+            const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+            const auto of = [&](unsigned v) { return unsigned(__builtin_amdgcn_readlane(int(v), l)); };
+            const unsigned in = index - (items + of(to) - of(mine)), c = of(chunks);
+            Item it;
+            it.any = true;
+            it.request = r0 + l;
+            it.start = int(of(unsigned(start)));
+            it.n = int(of(unsigned(n)));
+            it.len = int(of(unsigned(len)));
+            it.tile = int(in / c);
+            it.chunk = int(in % c);
+            it.chunks = int(c);
+            it.step0 = it.chunk * int(per);
+            it.step1 = c == 1 ? 0x7FFFFFFF : it.step0 + int(per);
+            it.split = splits + of(sto) - of(split) + unsigned(it.tile) * c;
+            return it;
+        }
+        items += unsigned(__builtin_amdgcn_readlane(int(to), kWave - 1));
+        splits += unsigned(__builtin_amdgcn_readlane(int(sto), kWave - 1));
+    }
+    Item none{};
+    return none;
+}
+
+// ---- partials: [kTile][dim + 2] f32, the last two a row's maximum and sum ---------------------------
+// They pass between compute units of different L2s, so they are written and read as device-scope atomics,
+// 8 bytes each, which need no write-back of an L2; a counter of arrivals orders them.
+
+__device__ __forceinline__ void putPair(float *p, float a, float b) {
+    const uint64_t v = (uint64_t(__float_as_uint(b)) << 32) | __float_as_uint(a);
+    __hip_atomic_store(reinterpret_cast<uint64_t *>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t getPair(const float *p) {
+    return __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float firstOf(uint64_t v) { return __uint_as_float(uint32_t(v)); }
+__device__ __forceinline__ float secondOf(uint64_t v) { return __uint_as_float(uint32_t(v >> 32)); }
+
+// After the whole block's partial stores: true for the block that is the last of `count` to come to the counter.
+__device__ __forceinline__ bool arriveLast(unsigned *counter, unsigned count, unsigned *shared) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // this wave's partials are where every compute unit sees them
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const unsigned before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (before == count - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *shared = before;
+    }
+    __syncthreads();
+    const bool last = *shared == count - 1;
+    __syncthreads();
+    return last;
+}
+
+// Weight of a state of maximum m in a merge of maximum top (a state without keys has -inf).
+__device__ __forceinline__ float mergeWeight(float m, float top) { return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top); }
+
+// Merge of `count` partials, `stride` apart from `first`, in order: calls done(row, c, o, m, l) with 8 channels from c
+// on of each valid row, o not yet divided by l.
+template <int kTile, int kThreads, typename Done>
+__device__ void mergePartials(const float *first, size_t stride, int count, int dim, int rows, Done &&done) {
+    const int slots = dim / 8;
+    for (int j = threadIdx.x; j < rows * slots; j += kThreads) {
+        const int row = j / slots, c = (j - row * slots) * 8;
+        const float *p = first + size_t(row) * (dim + 2);
+        float m = -INFINITY, l = 0.0f, o[8] = {};
+        for (int k0 = 0; k0 < count; k0 += 8) {
+            uint64_t ml[8], x[8][4];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (k0 + k >= count) continue;
+                const float *pk = p + size_t(k0 + k) * stride;
+                ml[k] = getPair(pk + dim);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[k][e] = getPair(pk + c + 2 * e);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (k0 + k >= count) continue;
+                const float mk = firstOf(ml[k]), top = fmaxf(m, mk);
+                const float wa = mergeWeight(m, top), wb = mergeWeight(mk, top);
+                l = l * wa + secondOf(ml[k]) * wb;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    o[2 * e] = o[2 * e] * wa + firstOf(x[k][e]) * wb;
+                    o[2 * e + 1] = o[2 * e + 1] * wa + secondOf(x[k][e]) * wb;
+                }
+                m = top;
+            }
+        }
+        done(row, c, o, m, l);
+    }
+}
+
+// Ends an item: `state(row, c, o, m, l)` gives 8 channels of the block's own result.  One chunk: the outputs.  Several: the
+// partial, and for the last of kFan chunks, and of those the last, the merge.
+template <typename T, int kTile, int kThreads, typename State>
+__device__ void finishItem(const PagedAttnArgs &a, const Item &it, int head, int first_row, int rows, unsigned *shared,
+                           State &&state) {
+    const int dim = a.dim, slots = dim / 8;
+    const auto put = [&](int row, int c, const float *o, float, float l) {
+        const int m = first_row + row, i = m / a.group;
+        const size_t at = (size_t(it.start + i) * a.nh + size_t(head) * a.group + (m - i * a.group)) * dim + c;
+        const float d = l == 0.0f ? 0.0f : 1.0f / l; // no key: 0 (l >= 2^15 where there is one)
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = o[e] * d;
+        store8<T>(a.out, at, f);
+    };
+    if (it.chunks == 1) {
+        for (int j = threadIdx.x; j < rows * slots; j += kThreads) {
+            const int row = j / slots, c = (j - row * slots) * 8;
+            float o[8], m, l;
+            state(row, c, o, m, l);
+            put(row, c, o, m, l);
+        }
+        return;
+    }
+    const size_t size = size_t(kTile) * (dim + 2), stride = size * a.heads;
+    const auto partial = [&](int chunk) { return a.part + (size_t(it.split + unsigned(chunk)) * a.heads + head) * size; };
+    const auto keep = [&](float *to) {
+        return [&, to](int row, int c, const float *o, float m, float l) {
+            float *p = to + size_t(row) * (dim + 2);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) putPair(p + c + 2 * e, o[2 * e], o[2 * e + 1]);
+            if (c == 0) putPair(p + dim, m, l);
+        };
+    };
+    const auto mine = keep(partial(it.chunk));
+    for (int j = threadIdx.x; j < rows * slots; j += kThreads) {
+        const int row = j / slots, c = (j - row * slots) * 8;
+        float o[8], m, l;
+        state(row, c, o, m, l);
+        mine(row, c, o, m, l);
+    }
+    const auto counter = [&](int level, int chunk) {
+        return a.arrived + size_t(level) * kPagedCounters + size_t(it.split + unsigned(chunk)) * a.heads + head;
+    };
+    const int group0 = it.chunk / kFan * kFan, in_group = min(kFan, it.chunks - group0);
+    if (!arriveLast(counter(0, group0), unsigned(in_group), shared)) return;
+    if (it.chunks <= kFan) {
+        mergePartials<kTile, kThreads>(partial(group0), stride, in_group, dim, rows, put);
+        return;
+    }
+    // the merge of a group, in a partial of its own
+    const int groups = (it.chunks + kFan - 1) / kFan;
+    float *merged = a.part + size_t(a.splits) * size;
+    const auto keepMerged = keep(merged + (size_t(it.split + unsigned(group0)) * a.heads + head) * size);
+    mergePartials<kTile, kThreads>(partial(group0), stride, in_group, dim, rows, keepMerged);
+    if (!arriveLast(counter(1, 0), unsigned(groups), shared)) return;
+    mergePartials<kTile, kThreads>(merged + (size_t(it.split) * a.heads + head) * size, stride * kFan, groups, dim, rows, put);
+}
+
+
+} // namespace llaisys::kernels

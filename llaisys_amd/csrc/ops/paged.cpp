@@ -158,16 +158,18 @@ void pagedAttentionInt8KV(tensor_t attn_val, tensor_t q, tensor_t k_cache, tenso
     const size_t requests = block_table->shape()[0], width = block_table->shape()[1];
     ASSERT(kv_lens->numel() == requests && row_starts->numel() == requests + 1,
            "PagedAttentionInt8KV: kv_lens must hold a length per request and row_starts requests + 1 elements");
-    ASSERT(rows < kLimit && requests < kLimit && width < kLimit && nh <= 65535,
-           "PagedAttentionInt8KV: sizes must be below 2^31, heads at most 65535");
+    ASSERT(rows < kLimit && requests < kLimit && nh <= 65535, "PagedAttentionInt8KV: sizes must be below 2^31, heads at most 65535");
+    ASSERT(width < kLimit && width * c.block <= kLimit - 4096, "PagedAttentionInt8KV: a request's blocks must hold fewer than 2^31 tokens");
     ASSERT(!overlaps(attn_val, q), "PagedAttentionInt8KV: attn_val must not overlap q");
     requireAligned(q, op);
     requireAligned(attn_val, op);
     auto s = streamFor(q);
-    kernels::pagedAttentionInt8KV({attn_val->data(), q->data(), c, ptr<const int32_t>(block_table),
-                                   ptr<const int32_t>(row_starts), ptr<const int32_t>(kv_lens), rows, requests, width, nh,
-                                   scale, q->dtype(), device::amd::errorWord(q->deviceId())},
-                                  s);
+    const kernels::PagedAttentionCall call{attn_val->data(), q->data(), c, ptr<const int32_t>(block_table),
+                                           ptr<const int32_t>(row_starts), ptr<const int32_t>(kv_lens), rows, requests, width,
+                                           nh, scale, q->dtype(), device::amd::errorWord(q->deviceId())};
+    const size_t want = kernels::pagedAttentionWorkspaceBytes(call);
+    void *ws = want ? device::amd::tryWorkspace(q->deviceId(), kernels::kScratchReserved + want, s) : nullptr;
+    kernels::pagedAttentionInt8KV(call, ws, want, s);
     launched("pagedAttentionInt8KV");
 }
 
