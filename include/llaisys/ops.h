@@ -174,7 +174,8 @@ __C {
     /* ---- KV cache in blocks, for many requests at once (no reference counterpart: its decoder
      * keeps one contiguous cache per layer for one sequence, src/models/qwen2/attention.hpp:108-123).
      * k_cache, v_cache [n_blocks, n_kvh, block, d] I8 and k_scale, v_scale [n_blocks, n_kvh] F32: a
-     * value is code * scale of its block and head.  block is a power of two in [16, 256], d a multiple
+     * value is code * scale of its block and head (scales are finite and not negative; another makes
+     * NaN of its values).  block is a power of two in [16, 256], d a multiple
      * of 16 up to 256.  block_table [requests, width] I32 holds each request's block ids in order; a
      * token's slot is block id * block + offset.  What the device finds out of range is skipped and
      * reported through llaisysTakeDeviceError (4); nothing outside the tensors is read or written. */

@@ -75,20 +75,21 @@ __global__ __launch_bounds__(NW *kWave, NT <= 2 ? 2 : 1) void pagedFew(PagedAttn
 
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave), lane = int(threadIdx.x) % kWave;
     const int m16 = lane % 16, quarter = lane / 16, head = int(blockIdx.y);
-    const Item it = findItem<kRows>(a, blockIdx.x, NW, blockIdx.x == 0 && head == 0 && wave == 0);
+    Item it = findItem<kRows>(a, blockIdx.x, NW, blockIdx.x == 0 && head == 0 && wave == 0);
     if (!it.any) return;
 
     const int first_row = it.tile * kRows, rows = int(min(int64_t(kRows), int64_t(it.n) * a.group - first_row));
     const int row = first_row + m16, token = row / a.group;
     const int before = it.len - it.n; // tokens cached before the rows; a row sees before + token + 1
     const int seen_last = before + (first_row + rows - 1) / a.group + 1, seen_first = before + first_row / a.group + 1;
+    const int steps = seen_last > 0 ? (seen_last + kStep - 1) / kStep : 0;
+    if (!cutItem(it, steps)) return;
+    const int end = min(it.step1, steps);
     const int limit = before + token + 1;
     QueryRows<T, NT> q;
     q.load(a, m16 < rows, (size_t(it.start + token) * a.nh + size_t(head) * a.group + (row - token * a.group)) * dim, quarter);
     const float row_scale = __builtin_amdgcn_ldexpf(a.scale * kLog2e, 9 - q.exponent);
 
-    const int steps = seen_last > 0 ? (seen_last + kStep - 1) / kStep : 0;
-    const int end = min(it.step1, steps);
     const int32_t *table = a.table + it.request * a.width;
     const int in_block = (1 << a.shift) - 1;
     const size_t tile_bytes = size_t(dim) << a.shift;
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(NW *kWave, NT <= 2 ? 2 : 1) void pagedFew(PagedAttn
                 }
             }
         }
-        const float c = row_scale * d.ks;
+        const float c = row_scale * checkedScale(d.ks);
         const int key0 = step * kStep + 16 * quarter;
         const bool some_hidden = __any(d.bad) || (step + 1) * kStep > seen_first;
         float top = mx;
@@ -159,8 +160,7 @@ __global__ __launch_bounds__(NW *kWave, NT <= 2 ? 2 : 1) void pagedFew(PagedAttn
             }
         top = butterflyStep<16, MaxOp>(top);
         top = butterflyStep<32, MaxOp>(top);
-        // a scale that is not finite makes its values NaN; it is no reference for the others
-        const float vs = d.vs < INFINITY ? d.vs : __builtin_nanf("");
+        const float vs = checkedScale(d.vs);
         float vtop = d.bad || key0 >= limit ? vref : fmaxf(vref, vs);
         vtop = butterflyStep<16, MaxOp>(vtop);
         vtop = butterflyStep<32, MaxOp>(vtop);
@@ -279,32 +279,43 @@ void launchFew(const PagedAttnArgs &a, unsigned items, hipStream_t s) {
 }
 
 constexpr unsigned kTarget = 512; // chunks over all heads: two blocks on each of 256 compute units
-constexpr int kFewRows = 16;
 
 struct Plan {
+    bool many;
+    int tile;
     size_t items, splits;
     unsigned target;
 };
 Plan planOf(const PagedAttentionCall &c) {
-    const size_t h = c.cache.heads, group = c.nh / h;
-    const size_t tiles = (c.rows * group) / kFewRows + std::min(c.rows, c.requests);
-    const size_t most = (c.width * c.cache.block + kStep - 1) / kStep, waves = c.cache.dim > 128 ? 2 : 4;
-    Plan p{tiles, 0, 0};
+    const size_t h = c.cache.heads, group = c.nh / h, requests = std::min(c.rows, c.requests);
+    Plan p{};
+    p.many = c.rows * group > 32 * requests;
+    p.tile = p.many ? kPagedManyRows : 16;
+    const size_t tiles = c.rows * group / p.tile + requests;
+    const size_t most = (c.width * c.cache.block + kStep - 1) / kStep, least = !p.many && c.cache.dim > 128 ? 2 : 4;
+    p.items = tiles;
     const size_t per_head = (kTarget + h - 1) / h;
-    if (2 * per_head * h <= kPagedCounters && most > waves) {
+    if (2 * per_head * h <= kPagedCounters && most > least) {
         // sum of chunks <= tiles + steps / steps of a chunk; split tiles have at most twice the latter
         p.target = kTarget;
-        p.items = std::min(tiles + per_head, tiles * ((most + waves - 1) / waves));
+        p.items = std::min(tiles + per_head, tiles * ((most + least - 1) / least));
         p.splits = 2 * per_head * h;
     }
     return p;
+}
+
+template <typename T>
+void launch(const PagedAttnArgs &a, const Plan &p, hipStream_t s) {
+    if (p.many) launchPagedMany<T>(a, unsigned(p.items), s);
+    else launchFew<T>(a, unsigned(p.items), s);
 }
 
 } // namespace
 
 size_t pagedAttentionWorkspaceBytes(const PagedAttentionCall &c) {
     if (c.rows == 0 || c.requests == 0) return 0;
-    return 2 * planOf(c).splits * kFewRows * (c.cache.dim + 2) * sizeof(float);
+    const Plan p = planOf(c);
+    return 2 * p.splits * p.tile * (c.cache.dim + 2) * sizeof(float);
 }
 
 void pagedAttentionInt8KV(const PagedAttentionCall &c, void *ws, size_t ws_bytes, hipStream_t s) {
@@ -318,9 +329,9 @@ void pagedAttentionInt8KV(const PagedAttentionCall &c, void *ws, size_t ws_bytes
                           int64_t(c.cache.n_blocks), int(c.nh), int(c.cache.heads), int(c.nh / c.cache.heads), int(c.cache.dim),
                           __builtin_ctzll(c.cache.block), c.scale, c.err};
     switch (c.dt) {
-    case LLAISYS_DTYPE_F32: return launchFew<F32>(a, unsigned(p.items), s);
-    case LLAISYS_DTYPE_BF16: return launchFew<BF16>(a, unsigned(p.items), s);
-    case LLAISYS_DTYPE_F16: return launchFew<F16>(a, unsigned(p.items), s);
+    case LLAISYS_DTYPE_F32: return launch<F32>(a, p, s);
+    case LLAISYS_DTYPE_BF16: return launch<BF16>(a, p, s);
+    case LLAISYS_DTYPE_F16: return launch<F16>(a, p, s);
     default: return;
     }
 }

@@ -66,6 +66,9 @@ __device__ __forceinline__ v8h codes8(uint32_t lo, uint32_t hi) {
                        codePair(__builtin_amdgcn_perm(hi, hi, 0x0c010c00u)), codePair(__builtin_amdgcn_perm(hi, hi, 0x0c030c02u))}});
 }
 
+// Scales are finite and not negative; another makes NaN of what it scales, and of nothing else.
+__device__ __forceinline__ float checkedScale(float s) { return s >= 0.0f && s < INFINITY ? s : __builtin_nanf(""); }
+
 // f32 -> f16, to nearest; what it leaves over, again in f16.
 __device__ __forceinline__ v8h narrow8(const float *f) {
     v8h h;
@@ -184,12 +187,12 @@ __device__ Item findItem(const PagedAttnArgs &a, unsigned index, int per_chunk, 
             it.start = int(of(unsigned(start)));
             it.n = int(of(unsigned(n)));
             it.len = int(of(unsigned(len)));
-            it.tile = int(in / c);
+            it.tile = int(of(tiles)) - 1 - int(in / c); // the last sees most keys: first
             it.chunk = int(in % c);
             it.chunks = int(c);
             it.step0 = it.chunk * int(per);
             it.step1 = c == 1 ? 0x7FFFFFFF : it.step0 + int(per);
-            it.split = splits + of(sto) - of(split) + unsigned(it.tile) * c;
+            it.split = splits + of(sto) - of(split) + in / c * c;
             return it;
         }
         items += unsigned(__builtin_amdgcn_readlane(int(to), kWave - 1));
@@ -327,5 +330,18 @@ __device__ void finishItem(const PagedAttnArgs &a, const Item &it, int head, int
     mergePartials<kTile, kThreads>(merged + (size_t(it.split) * a.heads + head) * size, stride * kFan, groups, dim, rows, put);
 }
 
+
+// Cuts the item to the `steps` its tile sees; false where its chunk has none of them (the tile's first chunk always runs).
+__device__ __forceinline__ bool cutItem(Item &it, int steps) {
+    if (it.chunks == 1) return true;
+    const int per = it.step1 - it.step0;
+    it.chunks = steps > per ? (steps + per - 1) / per : 1;
+    return it.chunk < it.chunks;
+}
+
+// Rows by the 128 a tile (paged_attention_many.hip).
+constexpr int kPagedManyRows = 128;
+template <typename T>
+void launchPagedMany(const PagedAttnArgs &a, unsigned items, hipStream_t s);
 
 } // namespace llaisys::kernels

@@ -1,0 +1,349 @@
+// Attention over the KV cache in blocks, tiles of 128 rows: prompts and chunks of prompts.
+//
+// Four waves of 32 rows share tiles of 64 keys.  Each wave reads 16 of the keys (one block id) a tile ahead,
+// widens their codes to f16 and writes them to LDS once for all: K as it is, V transposed by the byte permutes that widen
+// it.  Sᵀ = K Qᵀ and Oᵀ = Vᵀ Pᵀ run on v_mfma_f32_32x32x16_f16; K's rows enter in the order that makes a
+// lane's 16 scores those of 16 keys in a row, so that its weights are the second product's operand as they are.
+// Both LDS images are read 16 bytes a lane, their 16-byte columns xor-ed with bits of the row so that neither the
+// reads nor the writes meet in a bank.
+#include "paged_attention.hpp"
+
+namespace llaisys::kernels {
+
+namespace {
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+constexpr int kManyRows = 128, kManyWaves = 4, kManyThreads = kManyWaves * kWave;
+// Weights are 2^(t - m + 11): m stays while no score passes it by more than 2^4, so that few tiles rescale the sums.
+constexpr float kManyBits = 11.0f, kLazy = 4.0f;
+
+// Column of a 16-byte piece of a K row (key) and of a V row (channel) in LDS.
+template <int DP>
+__device__ __forceinline__ int kColumn(int key, int piece) {
+    // lanes of a read differ in bits 0, 1, 4, 2 of the key first
+    if constexpr (DP == 64)
+        return piece ^ (((key >> 1) & 1) | ((key >> 3) & 2) | (key & 4));
+    else
+        return piece ^ ((key & 3) | ((key >> 2) & 4) | ((key << 1) & 8));
+}
+__device__ __forceinline__ int vColumn(int channel, int piece) { return piece ^ (((channel >> 2) & 7) ^ ((channel << 1) & 4)); }
+
+template <int DP>
+struct Buffers {
+    v4u k[2][kStep][DP / 8];   // [key][8 channels]
+    v4u v[2][DP][kStep / 8];   // [channel][8 keys]
+    float ks[2][4], vs[2][4], lvs[2][4]; // of 16 keys: scales, and log2 of v's
+    int bad[2][4];             // their block id is none
+};
+template <int DP>
+union Shared {
+    Buffers<DP> in;
+    float out[kManyRows][DP + 4];
+};
+
+// Two blocks a compute unit where 256 registers hold a wave's rows.
+template <typename T, int DP>
+constexpr int kManyBlocks = DP <= 128 && !std::is_same_v<T, F32> ? 2 : 1;
+
+template <typename T, int DP, int D>
+__global__ __launch_bounds__(kManyThreads, (kManyBlocks<T, DP>)) void pagedMany(PagedAttnArgs a) {
+    constexpr bool kTwoQ = std::is_same_v<T, F32>, kTwoP = !std::is_same_v<T, BF16>;
+    constexpr int kSteps = DP / 16, kTiles = DP / 32;
+    constexpr int kK = DP / 64;                 // 16-byte pieces of K a lane brings per tile
+    constexpr int kV = DP <= 128 ? 1 : 2;       // units of 8 keys x 4 channels of V
+    const int dim = D ? D : a.dim;
+    __shared__ Shared<DP> sh;
+    __shared__ float sm[kManyRows], sl[kManyRows];
+    __shared__ unsigned arrived;
+
+    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave), lane = int(threadIdx.x) % kWave;
+    const int col = lane % 32, half = lane / 32, head = int(blockIdx.y);
+    Item it = findItem<kManyRows>(a, blockIdx.x, 4, blockIdx.x == 0 && head == 0 && wave == 0);
+    if (!it.any) return;
+
+    const int total_rows = it.n * a.group; // fits: the tile index does
+    const int first_row = it.tile * kManyRows, rows = min(kManyRows, total_rows - first_row);
+    const int before = it.len - it.n;
+    const auto seenBy = [&](int row) { return before + row / a.group + 1; };
+    const int seen_last = seenBy(first_row + rows - 1);
+    const int steps = seen_last > 0 ? (seen_last + kStep - 1) / kStep : 0;
+    if (!cutItem(it, steps)) return;
+    const int end = min(it.step1, steps);
+
+    // this wave's rows
+    const int wrow = first_row + 32 * wave, row = wrow + col, token = row / a.group;
+    const bool valid = row < total_rows;
+    const int limit = before + token + 1;
+    const int wave_last = wrow < total_rows ? seenBy(min(wrow + 31, total_rows - 1)) : 0, wave_first = seenBy(wrow);
+    v8h q[kSteps], ql[kTwoQ ? kSteps : 1];
+    float row_scale;
+    {
+        const size_t at = (size_t(it.start + token) * a.nh + size_t(head) * a.group + (row - token * a.group)) * dim + 8 * half;
+        const float sign = a.scale < 0.0f ? -1.0f : 1.0f; // the scale of a score is not negative below
+        float top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            float f[8] = {};
+            if (valid && 16 * s < dim) load8<T>(a.q, at + 16 * s, f);
+            top = foldFinite(top, f);
+        }
+        top = butterflyStep<32, MaxOp>(top);
+        const int e = rowExponent(top);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            float f[8] = {};
+            if (valid && 16 * s < dim) load8<T>(a.q, at + 16 * s, f); // again, from the cache: 8 values at a time in registers
+#pragma unroll
+            for (int x = 0; x < 8; ++x) f[x] = __builtin_amdgcn_ldexpf(sign * f[x], e);
+            q[s] = narrow8(f);
+            if constexpr (kTwoQ) ql[s] = rest8(f, q[s]);
+        }
+        row_scale = __builtin_amdgcn_ldexpf(fabsf(a.scale) * kLog2e, 9 - e);
+    }
+
+    // ---- the wave's 16 keys of a tile: HBM -> registers -> LDS
+    const int32_t *table = a.table + it.request * a.width;
+    const size_t tile_bytes = size_t(dim) << a.shift;
+    const int in_block = (1 << a.shift) - 1;
+    const int k_key = (lane * 16) / DP, k_piece = lane % (DP / 16); // i-th piece: key k_key + i * 1024 / DP
+    const int v_quad = (lane % (DP / 4 < kWave ? DP / 4 : kWave)), v_chunk = DP <= 128 ? lane / (DP / 4) : 0;
+    v4u kr[kK];
+    uint32_t vr[kV][8];
+    float ks = 0.0f, vs = 0.0f;
+    bool bad = false;
+    int id_next = 0;
+    const auto idOf = [&](int step) { return table[min(step * kStep + 16 * wave, seen_last - 1) >> a.shift]; };
+    const auto fetch = [&](int step) { // uses id_next, and reads the id after it
+        const int id = __builtin_amdgcn_readfirstlane(id_next);
+        bad = uint32_t(id) >= uint32_t(a.n_blocks);
+        if (bad && lane == 0 && step * kStep + 16 * wave < seen_last) atomicOr(a.err, kErrPagedIndex);
+        const int64_t tile = (bad ? 0 : int64_t(id)) * a.heads + head;
+        const size_t at = tile * tile_bytes + size_t((step * kStep + 16 * wave) & in_block) * dim;
+        const int8_t *kp = a.k_codes + at, *vp = a.v_codes + at;
+        int c = 16 * k_piece;
+        if (D != DP) c = c < dim ? c : 0; // behind the row: q is 0 there
+#pragma unroll
+        for (int i = 0; i < kK; ++i) kr[i] = *reinterpret_cast<const v4u *>(kp + unsigned((k_key + i * (1024 / DP)) * dim + c));
+        if (DP >= 128 || lane < 32) {
+#pragma unroll
+            for (int u = 0; u < kV; ++u) {
+                int ch = 4 * v_quad;
+                if (D != DP) ch = ch < dim ? ch : 0; // not stored
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    vr[u][i] = *reinterpret_cast<const uint32_t *>(vp + unsigned((8 * (v_chunk + u) + i) * dim + ch));
+            }
+        }
+        ks = a.k_scale[tile];
+        vs = a.v_scale[tile];
+        if (step + 1 < end) id_next = idOf(step + 1);
+    };
+    const auto stage = [&](int b) {
+        Buffers<DP> &s = sh.in;
+#pragma unroll
+        for (int i = 0; i < kK; ++i) {
+            const int key = 16 * wave + k_key + i * (1024 / DP);
+            s.k[b][key][kColumn<DP>(key, 2 * k_piece)] = __builtin_bit_cast(v4u, codes8(kr[i].x, kr[i].y));
+            s.k[b][key][kColumn<DP>(key, 2 * k_piece + 1)] = __builtin_bit_cast(v4u, codes8(kr[i].z, kr[i].w));
+        }
+        if (DP >= 128 || lane < 32) {
+#pragma unroll
+            for (int u = 0; u < kV; ++u) {
+                uint32_t v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = vr[u][i] ^ 0x80808080u;
+                constexpr uint32_t kSel[4] = {0x0c040c00u, 0x0c050c01u, 0x0c060c02u, 0x0c070c03u};
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    Pairs p;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p.p[e] = codePair(__builtin_amdgcn_perm(v[2 * e + 1], v[2 * e], kSel[x]));
+                    const int ch = 4 * v_quad + x;
+                    s.v[b][ch][vColumn(ch, 2 * wave + v_chunk + u)] = __builtin_bit_cast(v4u, join(p));
+                }
+            }
+        }
+        if (lane == 0) {
+            const float v = checkedScale(vs);
+            s.ks[b][wave] = checkedScale(ks);
+            s.vs[b][wave] = v;
+            s.lvs[b][wave] = __builtin_amdgcn_logf(v);
+            s.bad[b][wave] = bad;
+        }
+    };
+
+    // ---- one tile's products
+    float mx = -INFINITY, l = 0.0f, vref = 0.0f, lref = 0.0f;
+    v16f acc[kTiles];
+#pragma unroll
+    for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
+    const int my_key = 16 * (col / 4 % 2) + 4 * (col / 8) + col % 4; // K's row at this lane's place of the operand
+
+    const auto compute = [&](int step, int b) {
+        const Buffers<DP> &s = sh.in;
+        v16f sc[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[t][i] = 0.0f;
+            const int key = 32 * t + my_key;
+#pragma unroll
+            for (int x = 0; x < kSteps; ++x) {
+                const v8h k = __builtin_bit_cast(v8h, s.k[b][key][kColumn<DP>(key, 2 * x + half)]);
+                sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[x], sc[t], 0, 0, 0);
+                if constexpr (kTwoQ) sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[x], sc[t], 0, 0, 0);
+            }
+        }
+        // this lane's keys: 32 t + 16 half + 0..15
+        float kscale[2], vscale[2], lv[2];
+        bool none[2], hide = (step + 1) * kStep > wave_first, zero = false;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            hide = hide || s.bad[b][g] != 0;
+            zero = zero || s.vs[b][g] == 0.0f;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            kscale[t] = s.ks[b][2 * t + half];
+            vscale[t] = s.vs[b][2 * t + half];
+            lv[t] = s.lvs[b][2 * t + half];
+            none[t] = s.bad[b][2 * t + half] != 0;
+        }
+        hide = __builtin_amdgcn_readfirstlane(hide);
+        zero = __builtin_amdgcn_readfirstlane(zero);
+        float c[2], top = -INFINITY, vtop = vref;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int key0 = step * kStep + 32 * t + 16 * half;
+            c[t] = row_scale * kscale[t];
+            if (hide) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (none[t] || key0 + i >= limit) sc[t][i] = -INFINITY;
+            }
+            float best = sc[t][0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) best = fmaxf(best, sc[t][i]);
+            top = fmaxf(top, best * c[t]);
+            vtop = hide && (none[t] || key0 >= limit) ? vtop : fmaxf(vtop, vscale[t]);
+        }
+        top = butterflyStep<32, MaxOp>(top);
+        vtop = butterflyStep<32, MaxOp>(vtop);
+        if (__any(top > mx + kLazy || vtop > vref || (mx == -INFINITY && top > mx))) {
+            const float m = fmaxf(mx, top), keep = mergeWeight(mx, m);
+            const float f = vtop > vref ? keep * (vref / vtop) : keep;
+            l *= keep;
+#pragma unroll
+            for (int k = 0; k < kTiles; ++k) acc[k] *= f;
+            mx = m;
+            vref = vtop;
+            lref = vref > 0.0f ? __builtin_amdgcn_logf(vref) : 0.0f;
+        }
+        const float base = (mx == -INFINITY ? 0.0f : mx) - kManyBits;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            v8h p[2], r[2];
+            float sum = 0.0f;
+            if (kTwoQ || zero || hide) {
+                const float w = vref > 0.0f ? vscale[t] / vref : vscale[t]; // 0, or NaN, where no scale was above 0
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float f[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float x = sc[t][8 * u + e];
+                        const bool out = hide && x == -INFINITY;
+                        const float y = out ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(x, c[t], -base));
+                        sum += y;
+                        f[e] = out ? 0.0f : y * w;
+                    }
+                    p[u] = narrow8(f);
+                    if constexpr (kTwoP) r[u] = rest8(f, p[u]);
+                }
+            } else {
+                // the value scale's ratio goes into the exponent, and out of the sum at once
+                const float shift = lv[t] - lref, to = base - shift;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float f[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        f[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][8 * u + e], c[t], -to));
+                        sum += f[e];
+                    }
+                    p[u] = narrow8(f);
+                    if constexpr (kTwoP) r[u] = rest8(f, p[u]);
+                }
+                sum *= __builtin_amdgcn_exp2f(-shift);
+            }
+            l += sum;
+#pragma unroll
+            for (int k = 0; k < kTiles; ++k) {
+                const int ch = 32 * k + col;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const v8h v = __builtin_bit_cast(v8h, s.v[b][ch][vColumn(ch, 4 * t + 2 * half + u)]);
+                    acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[u], acc[k], 0, 0, 0);
+                    if constexpr (kTwoP) acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, r[u], acc[k], 0, 0, 0);
+                }
+            }
+        }
+    };
+
+    if (it.step0 < end) {
+        id_next = idOf(it.step0);
+        fetch(it.step0);
+        stage(0);
+        if (it.step0 + 1 < end) fetch(it.step0 + 1);
+        ldsBarrier();
+        for (int step = it.step0, b = 0; step < end; ++step, b ^= 1) {
+            if (step + 1 < end) stage(b ^ 1);
+            if (step + 2 < end) fetch(step + 2);
+            if (step * kStep < wave_last) compute(step, b);
+            ldsBarrier();
+        }
+    }
+
+    // ---- outputs through LDS: row, 8 channels
+    l = butterflyStep<32, SumOp>(l);
+    const float unit = vref * (1.0f / kCodeUnit);
+    const int mine = 32 * wave + col;
+#pragma unroll
+    for (int k = 0; k < kTiles; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int ch = 32 * k + 8 * (i / 4) + 4 * half;
+            *reinterpret_cast<v4f *>(&sh.out[mine][ch]) = v4f{acc[k][i] * unit, acc[k][i + 1] * unit, acc[k][i + 2] * unit, acc[k][i + 3] * unit};
+        }
+    if (half == 0) {
+        sm[mine] = mx;
+        sl[mine] = l;
+    }
+    __syncthreads();
+    finishItem<T, kManyRows, kManyThreads>(a, it, head, first_row, rows, &arrived, [&](int r, int c, float *o, float &m, float &sum) {
+        m = sm[r];
+        sum = sl[r];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = sh.out[r][c + e];
+    });
+}
+
+} // namespace
+
+template <typename T>
+void launchPagedMany(const PagedAttnArgs &a, unsigned items, hipStream_t s) {
+    const dim3 grid(items, unsigned(a.heads));
+    if (a.dim == 128) pagedMany<T, 128, 128><<<grid, kManyThreads, 0, s>>>(a);
+    else if (a.dim == 64) pagedMany<T, 64, 64><<<grid, kManyThreads, 0, s>>>(a);
+    else if (a.dim < 64) pagedMany<T, 64, 0><<<grid, kManyThreads, 0, s>>>(a);
+    else if (a.dim < 128) pagedMany<T, 128, 0><<<grid, kManyThreads, 0, s>>>(a);
+    else pagedMany<T, 256, 0><<<grid, kManyThreads, 0, s>>>(a);
+}
+template void launchPagedMany<F32>(const PagedAttnArgs &, unsigned, hipStream_t);
+template void launchPagedMany<BF16>(const PagedAttnArgs &, unsigned, hipStream_t);
+template void launchPagedMany<F16>(const PagedAttnArgs &, unsigned, hipStream_t);
+
+} // namespace llaisys::kernels
