@@ -1,9 +1,10 @@
 // Shared by the kernels of the attention over the KV cache in blocks (paged_attention*.hip).
 //
 // The rows of a request and a kv head are its n tokens times the group = nh / heads q heads that share the
-// kv head: row m is token m / group, head m % group of the group.  A tile of rows attends its keys in steps
-// of 64; where the tiles of all requests would leave compute units idle, the keys are split into chunks of a
-// whole number of steps, and whoever finishes a tile's last chunk merges them.
+// kv head: row m is token m / group, head m % group of the group.  Requests of few rows are attended in
+// tiles of 16 rows (paged_attention_few.hpp), others in tiles of 128 (paged_attention_many.hpp).  A tile attends its
+// keys in steps of 64; where the tiles of all requests would leave compute units idle, the keys
+// are split into chunks of a whole number of steps, and whoever finishes a tile's last chunk merges them.
 //
 // Codes meet the matrix instructions as f16: a code is a whole number of magnitude <= 127, exact in f16, for
 // every element type of q.  Rows of q are multiplied by a power of two that brings their largest element to
@@ -19,8 +20,12 @@
 
 namespace llaisys::kernels {
 
-constexpr int kStep = 64;    // keys of a step
-constexpr int kFan = 16;     // chunks merged at once
+constexpr int kStep = 64;          // keys of a step
+constexpr int kFan = 16;           // chunks merged at once
+constexpr int kPagedThreads = 256; // of a block
+constexpr int kFewTile = 16, kManyTile = 128;
+constexpr int kFewMost = 32;       // rows of a request that go by 16, next to others that do not
+constexpr int kLeast = 4;          // steps of a chunk: a multiple of this
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kCodeUnit = 0x1p-9f; // a code's f16 value is code * kCodeUnit
 constexpr float kWeightBits = 15.0f; // weights are 2^(t - m + kWeightBits)
@@ -31,10 +36,10 @@ struct PagedAttnArgs {
     const int8_t *k_codes, *v_codes;
     const float *k_scale, *v_scale;
     const int32_t *table, *starts, *lens;
-    float *part;        // [2][splits] partials: of chunks, of groups of chunks
+    float *part;        // partials of chunks of split tiles
     unsigned *arrived;  // [2][kPagedCounters], 0 between launches
-    unsigned splits;
     unsigned target;    // chunks wanted over all requests and heads; 0: no tile is split
+    int few_most, many_least; // rows of the requests that the launch attends: up to, from
     int64_t rows, requests, width, n_blocks;
     int nh, heads, group, dim, shift;
     float scale;
@@ -117,34 +122,36 @@ __device__ __forceinline__ int rowExponent(float top) { return top > 0.0f ? 15 -
 // What a block of threads works at: a tile of one request's rows and a chunk of its keys.
 struct Item {
     bool any;
-    int64_t start;     // first row of the request in q
+    int start;         // first row of the request in q
     int64_t request;
     int n, len;        // rows and cached tokens of the request
     int tile;
     int step0, step1;  // steps of the chunk (not cut to what the tile sees)
     int chunk, chunks; // of the tile
-    unsigned split;    // partial of the tile's first chunk, where chunks > 1
+    unsigned split;    // number of the tile's first chunk among those of split tiles, where chunks > 1
 };
 
 // The item of index `index`: requests in order, of each its tiles, of each its chunks.  Every wave finds it by
 // itself: sums over the requests 64 at a time, so that no table of items has to be made before.
 template <int kTile>
-__device__ Item findItem(const PagedAttnArgs &a, unsigned index, int per_chunk, bool report) {
+__device__ __forceinline__ Item findItem(const PagedAttnArgs &a, unsigned index, bool report) {
     const int lane = threadIdx.x % kWave;
     const auto request = [&](int64_t r, int &start, int &n, int &len) { // false: out of range, skipped
         start = n = len = 0;
         if (r >= a.requests) return true;
         const int64_t s0 = a.starts[r], s1 = a.starts[r + 1], k = a.lens[r];
         if (s0 < 0 || s1 < s0 || s1 > a.rows || k < 0 || k > (a.width << a.shift)) return false;
+        const int rows = int(s1 - s0) * a.group;
+        if (rows > a.few_most || rows < a.many_least) return true; // another launch's
         start = int(s0);
         n = int(s1 - s0);
         len = int(k);
         return true;
     };
-    const auto tilesOf = [&](int n) { return unsigned((int64_t(n) * a.group + kTile - 1) / kTile); };
-    const auto stepsOf = [&](int len) { return unsigned((int64_t(len) + kStep - 1) / kStep); };
-    // steps of a chunk
-    unsigned per = 0x7FFFFFFFu;
+    const auto tilesOf = [&](int n) { return (unsigned(n * a.group) + kTile - 1) / kTile; };
+    const auto stepsOf = [&](int len) { return (unsigned(len) + kStep - 1) / kStep; };
+    constexpr unsigned kAll = 0x7FFFFFFFu;
+    unsigned per = kAll; // steps of a chunk
     int start, n, len;
     if (a.target || report) {
         uint64_t total = 0;
@@ -160,16 +167,16 @@ __device__ Item findItem(const PagedAttnArgs &a, unsigned index, int per_chunk, 
         // row starts that go back may make more items than the grid has: a tile whose chunks did not all run
         // would leave its counter behind, so nothing is split then
         if (a.target && fine) {
-            const uint64_t want = (total * unsigned(a.heads) + a.target - 1) / a.target;
-            const uint64_t up = (want + per_chunk - 1) / per_chunk * per_chunk;
-            per = up < per_chunk ? unsigned(per_chunk) : (up < per ? unsigned(up) : per);
+            const uint64_t want = (total * unsigned(a.heads) + a.target - 1) / a.target, up = (want + kLeast - 1) / kLeast * kLeast;
+            per = up < kLeast ? kLeast : (up < kAll ? unsigned(up) : kAll);
         }
     }
     unsigned items = 0, splits = 0; // before this group of requests
     for (int64_t r0 = 0; r0 < a.requests; r0 += kWave) {
         request(r0 + lane, start, n, len);
         const unsigned tiles = tilesOf(n), steps = stepsOf(len), chunks = steps > per ? (steps + per - 1) / per : 1;
-        unsigned mine = tiles * chunks, split = chunks > 1 ? mine : 0, to = mine, sto = split;
+        const unsigned mine = tiles * chunks, split = chunks > 1 ? mine : 0;
+        unsigned to = mine, sto = split;
 #pragma unroll
         for (int d = 1; d < kWave; d <<= 1) {
             const unsigned u = __shfl_up(to, d, kWave), v = __shfl_up(sto, d, kWave);
@@ -180,29 +187,40 @@ __device__ Item findItem(const PagedAttnArgs &a, unsigned index, int per_chunk, 
         if (hit) {
             const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
             const auto of = [&](unsigned v) { return unsigned(__builtin_amdgcn_readlane(int(v), l)); };
-            const unsigned in = index - (items + of(to) - of(mine)), c = of(chunks);
+            const unsigned in = index - (items + of(to - mine)), c = of(chunks), t = in / c;
             Item it;
             it.any = true;
             it.request = r0 + l;
             it.start = int(of(unsigned(start)));
             it.n = int(of(unsigned(n)));
             it.len = int(of(unsigned(len)));
-            it.tile = int(of(tiles)) - 1 - int(in / c); // the last sees most keys: first
-            it.chunk = int(in % c);
+            it.tile = int(of(tiles) - 1 - t); // the last sees most keys: first
+            it.chunk = int(in - t * c);
             it.chunks = int(c);
             it.step0 = it.chunk * int(per);
-            it.step1 = c == 1 ? 0x7FFFFFFF : it.step0 + int(per);
-            it.split = splits + of(sto) - of(split) + in / c * c;
+            it.step1 = c == 1 ? int(kAll) : it.step0 + int(per);
+            it.split = splits + of(sto - split) + t * c;
             return it;
         }
-        items += unsigned(__builtin_amdgcn_readlane(int(to), kWave - 1));
-        splits += unsigned(__builtin_amdgcn_readlane(int(sto), kWave - 1));
+        const auto last = [](unsigned v) { return unsigned(__builtin_amdgcn_readlane(int(v), kWave - 1)); };
+        items += last(to);
+        splits += last(sto);
     }
     Item none{};
     return none;
 }
 
-// ---- partials: [kTile][dim + 2] f32, the last two a row's maximum and sum ---------------------------
+// Cuts the item to the `steps` its tile sees; false where its chunk has none of them (the tile's first chunk always runs).
+__device__ __forceinline__ bool cutItem(Item &it, int steps) {
+    if (it.chunks == 1) return true;
+    const int per = it.step1 - it.step0;
+    it.chunks = steps > per ? (steps + per - 1) / per : 1;
+    return it.chunk < it.chunks;
+}
+
+// ---- partials: [rows of a tile][dim + 4] f32 ---------------------------------------------------
+// 8 channels at a time; behind them a row's maximum and sum, those of the chunk and those of the group of chunks whose
+// merge lies where its first chunk was (each thread overwrites the channels that it alone read).
 // They pass between compute units of different L2s, so they are written and read as device-scope atomics,
 // 8 bytes each, which need no write-back of an L2; a counter of arrivals orders them.
 
@@ -235,13 +253,13 @@ __device__ __forceinline__ bool arriveLast(unsigned *counter, unsigned count, un
 __device__ __forceinline__ float mergeWeight(float m, float top) { return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top); }
 
 // Merge of `count` partials, `stride` apart from `first`, in order: calls done(row, c, o, m, l) with 8 channels from c
-// on of each valid row, o not yet divided by l.
-template <int kTile, int kThreads, typename Done>
-__device__ void mergePartials(const float *first, size_t stride, int count, int dim, int rows, Done &&done) {
+// on of each valid row, o not yet divided by l.  `level`: of chunks (0), of groups (1).
+template <typename Done>
+__device__ __forceinline__ void mergePartials(const float *first, size_t stride, int count, int level, int dim, int rows, Done &&done) {
     const int slots = dim / 8;
-    for (int j = threadIdx.x; j < rows * slots; j += kThreads) {
+    for (int j = threadIdx.x; j < rows * slots; j += kPagedThreads) {
         const int row = j / slots, c = (j - row * slots) * 8;
-        const float *p = first + size_t(row) * (dim + 2);
+        const float *p = first + size_t(row) * (dim + 4);
         float m = -INFINITY, l = 0.0f, o[8] = {};
         for (int k0 = 0; k0 < count; k0 += 8) {
             uint64_t ml[8], x[8][4];
@@ -249,7 +267,7 @@ __device__ void mergePartials(const float *first, size_t stride, int count, int 
             for (int k = 0; k < 8; ++k) {
                 if (k0 + k >= count) continue;
                 const float *pk = p + size_t(k0 + k) * stride;
-                ml[k] = getPair(pk + dim);
+                ml[k] = getPair(pk + dim + 2 * level);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[k][e] = getPair(pk + c + 2 * e);
             }
@@ -273,74 +291,61 @@ __device__ void mergePartials(const float *first, size_t stride, int count, int 
 
 // Ends an item: `state(row, c, o, m, l)` gives 8 channels of the block's own result.  One chunk: the outputs.  Several: the
 // partial, and for the last of kFan chunks, and of those the last, the merge.
-template <typename T, int kTile, int kThreads, typename State>
-__device__ void finishItem(const PagedAttnArgs &a, const Item &it, int head, int first_row, int rows, unsigned *shared,
-                           State &&state) {
+template <typename T, int kTile, typename State>
+__device__ __forceinline__ void finishItem(const PagedAttnArgs &a, const Item &it, int head, int first_row, int rows, unsigned *shared,
+                                           State &&state) {
     const int dim = a.dim, slots = dim / 8;
     const auto put = [&](int row, int c, const float *o, float, float l) {
         const int m = first_row + row, i = m / a.group;
         const size_t at = (size_t(it.start + i) * a.nh + size_t(head) * a.group + (m - i * a.group)) * dim + c;
-        const float d = l == 0.0f ? 0.0f : 1.0f / l; // no key: 0 (l >= 2^15 where there is one)
+        const float d = l == 0.0f ? 0.0f : 1.0f / l; // no key: 0
         float f[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] = o[e] * d;
         store8<T>(a.out, at, f);
     };
-    if (it.chunks == 1) {
-        for (int j = threadIdx.x; j < rows * slots; j += kThreads) {
+    const auto all = [&](auto &&done) {
+        for (int j = threadIdx.x; j < rows * slots; j += kPagedThreads) {
             const int row = j / slots, c = (j - row * slots) * 8;
             float o[8], m, l;
             state(row, c, o, m, l);
-            put(row, c, o, m, l);
+            done(row, c, o, m, l);
         }
+    };
+    if (it.chunks == 1) {
+        all(put);
         return;
     }
-    const size_t size = size_t(kTile) * (dim + 2), stride = size * a.heads;
-    const auto partial = [&](int chunk) { return a.part + (size_t(it.split + unsigned(chunk)) * a.heads + head) * size; };
-    const auto keep = [&](float *to) {
-        return [&, to](int row, int c, const float *o, float m, float l) {
-            float *p = to + size_t(row) * (dim + 2);
+    const size_t size = size_t(kTile) * (dim + 4), stride = size * a.heads;
+    float *const base = a.part + (size_t(it.split) * a.heads + head) * size; // of the tile's first chunk
+    const auto keep = [&](int chunk, int level) {
+        float *to = base + size_t(chunk) * stride;
+        return [&, to, level](int row, int c, const float *o, float m, float l) {
+            float *p = to + size_t(row) * (dim + 4);
 #pragma unroll
             for (int e = 0; e < 4; ++e) putPair(p + c + 2 * e, o[2 * e], o[2 * e + 1]);
-            if (c == 0) putPair(p + dim, m, l);
+            if (c == 0) putPair(p + dim + 2 * level, m, l);
         };
     };
-    const auto mine = keep(partial(it.chunk));
-    for (int j = threadIdx.x; j < rows * slots; j += kThreads) {
-        const int row = j / slots, c = (j - row * slots) * 8;
-        float o[8], m, l;
-        state(row, c, o, m, l);
-        mine(row, c, o, m, l);
-    }
+    all(keep(it.chunk, 0));
     const auto counter = [&](int level, int chunk) {
         return a.arrived + size_t(level) * kPagedCounters + size_t(it.split + unsigned(chunk)) * a.heads + head;
     };
     const int group0 = it.chunk / kFan * kFan, in_group = min(kFan, it.chunks - group0);
     if (!arriveLast(counter(0, group0), unsigned(in_group), shared)) return;
+    const float *group = base + size_t(group0) * stride;
     if (it.chunks <= kFan) {
-        mergePartials<kTile, kThreads>(partial(group0), stride, in_group, dim, rows, put);
+        mergePartials(group, stride, in_group, 0, dim, rows, put);
         return;
     }
-    // the merge of a group, in a partial of its own
     const int groups = (it.chunks + kFan - 1) / kFan;
-    float *merged = a.part + size_t(a.splits) * size;
-    const auto keepMerged = keep(merged + (size_t(it.split + unsigned(group0)) * a.heads + head) * size);
-    mergePartials<kTile, kThreads>(partial(group0), stride, in_group, dim, rows, keepMerged);
+    mergePartials(group, stride, in_group, 0, dim, rows, keep(group0, 1));
     if (!arriveLast(counter(1, 0), unsigned(groups), shared)) return;
-    mergePartials<kTile, kThreads>(merged + (size_t(it.split) * a.heads + head) * size, stride * kFan, groups, dim, rows, put);
+    mergePartials(base, stride * kFan, groups, 1, dim, rows, put);
 }
 
-
-// Cuts the item to the `steps` its tile sees; false where its chunk has none of them (the tile's first chunk always runs).
-__device__ __forceinline__ bool cutItem(Item &it, int steps) {
-    if (it.chunks == 1) return true;
-    const int per = it.step1 - it.step0;
-    it.chunks = steps > per ? (steps + per - 1) / per : 1;
-    return it.chunk < it.chunks;
-}
-
-// Rows by the 128 a tile (paged_attention_many.hip).
-constexpr int kPagedManyRows = 128;
+template <typename T>
+void launchPagedFew(const PagedAttnArgs &a, unsigned items, hipStream_t s);
 template <typename T>
 void launchPagedMany(const PagedAttnArgs &a, unsigned items, hipStream_t s);
 

@@ -6,15 +6,15 @@
 // lane's 16 scores those of 16 keys in a row, so that its weights are the second product's operand as they are.
 // Both LDS images are read 16 bytes a lane, their 16-byte columns xor-ed with bits of the row so that neither the
 // reads nor the writes meet in a bank.
+#pragma once
+
 #include "paged_attention.hpp"
 
 namespace llaisys::kernels {
 
-namespace {
-
 typedef float v16f __attribute__((ext_vector_type(16)));
 
-constexpr int kManyRows = 128, kManyWaves = 4, kManyThreads = kManyWaves * kWave;
+static_assert(kManyTile == 32 * (kPagedThreads / kWave), "32 rows a wave");
 // Weights are 2^(t - m + 11): m stays while no score passes it by more than 2^4, so that few tiles rescale the sums.
 constexpr float kManyBits = 11.0f, kLazy = 4.0f;
 
@@ -37,33 +37,35 @@ struct Buffers {
     int bad[2][4];             // their block id is none
 };
 template <int DP>
-union Shared {
-    Buffers<DP> in;
-    float out[kManyRows][DP + 4];
+struct ManyShared {
+    union {
+        Buffers<DP> in;
+        float out[kManyTile][DP + 4];
+    };
+    float m[kManyTile], l[kManyTile];
 };
 
 // Two blocks a compute unit where 256 registers hold a wave's rows.
 template <typename T, int DP>
 constexpr int kManyBlocks = DP <= 128 && !std::is_same_v<T, F32> ? 2 : 1;
 
+// DP: the head size, rounded up to a size the tiles are made for; D: the head size where it is that size, else 0.
 template <typename T, int DP, int D>
-__global__ __launch_bounds__(kManyThreads, (kManyBlocks<T, DP>)) void pagedMany(PagedAttnArgs a) {
+__global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany(PagedAttnArgs a) {
     constexpr bool kTwoQ = std::is_same_v<T, F32>, kTwoP = !std::is_same_v<T, BF16>;
     constexpr int kSteps = DP / 16, kTiles = DP / 32;
     constexpr int kK = DP / 64;                 // 16-byte pieces of K a lane brings per tile
     constexpr int kV = DP <= 128 ? 1 : 2;       // units of 8 keys x 4 channels of V
-    const int dim = D ? D : a.dim;
-    __shared__ Shared<DP> sh;
-    __shared__ float sm[kManyRows], sl[kManyRows];
+    __shared__ ManyShared<DP> sh;
     __shared__ unsigned arrived;
-
+    const int dim = D ? D : a.dim;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave), lane = int(threadIdx.x) % kWave;
     const int col = lane % 32, half = lane / 32, head = int(blockIdx.y);
-    Item it = findItem<kManyRows>(a, blockIdx.x, 4, blockIdx.x == 0 && head == 0 && wave == 0);
+    Item it = findItem<kManyTile>(a, blockIdx.x, blockIdx.x == 0 && head == 0 && wave == 0);
     if (!it.any) return;
 
-    const int total_rows = it.n * a.group; // fits: the tile index does
-    const int first_row = it.tile * kManyRows, rows = min(kManyRows, total_rows - first_row);
+    const int total_rows = it.n * a.group;
+    const int first_row = it.tile * kManyTile, rows = min(kManyTile, total_rows - first_row);
     const int before = it.len - it.n;
     const auto seenBy = [&](int row) { return before + row / a.group + 1; };
     const int seen_last = seenBy(first_row + rows - 1);
@@ -319,31 +321,26 @@ __global__ __launch_bounds__(kManyThreads, (kManyBlocks<T, DP>)) void pagedMany(
             *reinterpret_cast<v4f *>(&sh.out[mine][ch]) = v4f{acc[k][i] * unit, acc[k][i + 1] * unit, acc[k][i + 2] * unit, acc[k][i + 3] * unit};
         }
     if (half == 0) {
-        sm[mine] = mx;
-        sl[mine] = l;
+        sh.m[mine] = mx;
+        sh.l[mine] = l;
     }
     __syncthreads();
-    finishItem<T, kManyRows, kManyThreads>(a, it, head, first_row, rows, &arrived, [&](int r, int c, float *o, float &m, float &sum) {
-        m = sm[r];
-        sum = sl[r];
+    finishItem<T, kManyTile>(a, it, head, first_row, rows, &arrived, [&](int r, int c, float *o, float &m, float &sum) {
+        m = sh.m[r];
+        sum = sh.l[r];
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[e] = sh.out[r][c + e];
     });
 }
 
-} // namespace
-
 template <typename T>
 void launchPagedMany(const PagedAttnArgs &a, unsigned items, hipStream_t s) {
     const dim3 grid(items, unsigned(a.heads));
-    if (a.dim == 128) pagedMany<T, 128, 128><<<grid, kManyThreads, 0, s>>>(a);
-    else if (a.dim == 64) pagedMany<T, 64, 64><<<grid, kManyThreads, 0, s>>>(a);
-    else if (a.dim < 64) pagedMany<T, 64, 0><<<grid, kManyThreads, 0, s>>>(a);
-    else if (a.dim < 128) pagedMany<T, 128, 0><<<grid, kManyThreads, 0, s>>>(a);
-    else pagedMany<T, 256, 0><<<grid, kManyThreads, 0, s>>>(a);
+    if (a.dim == 128) pagedMany<T, 128, 128><<<grid, kPagedThreads, 0, s>>>(a);
+    else if (a.dim == 64) pagedMany<T, 64, 64><<<grid, kPagedThreads, 0, s>>>(a);
+    else if (a.dim < 64) pagedMany<T, 64, 0><<<grid, kPagedThreads, 0, s>>>(a);
+    else if (a.dim < 128) pagedMany<T, 128, 0><<<grid, kPagedThreads, 0, s>>>(a);
+    else pagedMany<T, 256, 0><<<grid, kPagedThreads, 0, s>>>(a);
 }
-template void launchPagedMany<F32>(const PagedAttnArgs &, unsigned, hipStream_t);
-template void launchPagedMany<BF16>(const PagedAttnArgs &, unsigned, hipStream_t);
-template void launchPagedMany<F16>(const PagedAttnArgs &, unsigned, hipStream_t);
 
 } // namespace llaisys::kernels
