@@ -74,18 +74,21 @@ __device__ __forceinline__ v8h codes8(uint32_t lo, uint32_t hi) {
 // Scales are finite and not negative; another makes NaN of what it scales, and of nothing else.
 __device__ __forceinline__ float checkedScale(float s) { return s >= 0.0f && s < INFINITY ? s : __builtin_nanf(""); }
 
-// f32 -> f16, to nearest; what it leaves over, again in f16.
+// f32 -> f16, to nearest.
 __device__ __forceinline__ v8h narrow8(const float *f) {
     v8h h;
 #pragma unroll
     for (int e = 0; e < 8; ++e) h[e] = _Float16(f[e]);
     return h;
 }
-__device__ __forceinline__ v8h rest8(const float *f, const v8h &h) {
-    v8h l;
+// f in two f16 parts.  The first is made once: where the compiler sees both uses, it rounds a product straight to f16
+// for one (v_fma_mixlo) and over f32 for the other, which differ on ties, and the parts then do not add up.
+__device__ __forceinline__ void split8(const float *f, v8h &hi, v8h &lo) {
+    v4u bits = __builtin_bit_cast(v4u, narrow8(f));
+    asm("" : "+v"(bits));
+    hi = __builtin_bit_cast(v8h, bits);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) l[e] = _Float16(f[e] - float(h[e]));
-    return l;
+    for (int e = 0; e < 8; ++e) lo[e] = _Float16(f[e] - float(hi[e]));
 }
 
 template <typename T>
@@ -119,11 +122,13 @@ __device__ __forceinline__ float foldFinite(float m, const float *f) {
 // Exponent that brings `top` to [2^14, 2^15).
 __device__ __forceinline__ int rowExponent(float top) { return top > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0; }
 
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // What a block of threads works at: a tile of one request's rows and a chunk of its keys.
 struct Item {
     bool any;
     int start;         // first row of the request in q
-    int64_t request;
+    int request;
     int n, len;        // rows and cached tokens of the request
     int tile;
     int step0, step1;  // steps of the chunk (not cut to what the tile sees)
@@ -185,21 +190,22 @@ __device__ __forceinline__ Item findItem(const PagedAttnArgs &a, unsigned index,
         }
         const uint64_t hit = __ballot(index >= items + to - mine && index < items + to);
         if (hit) {
-            const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+            const int l = uniform(__ffsll(static_cast<unsigned long long>(hit)) - 1);
             const auto of = [&](unsigned v) { return unsigned(__builtin_amdgcn_readlane(int(v), l)); };
-            const unsigned in = index - (items + of(to - mine)), c = of(chunks), t = in / c;
+            const unsigned in = unsigned(uniform(int(index - items))) - of(to - mine), c = of(chunks), t = in / c;
+            // one value for the wave in every field: scalar registers, and branches that are no masks
             Item it;
             it.any = true;
-            it.request = r0 + l;
+            it.request = uniform(int(r0)) + l;
             it.start = int(of(unsigned(start)));
             it.n = int(of(unsigned(n)));
             it.len = int(of(unsigned(len)));
             it.tile = int(of(tiles) - 1 - t); // the last sees most keys: first
             it.chunk = int(in - t * c);
             it.chunks = int(c);
-            it.step0 = it.chunk * int(per);
-            it.step1 = c == 1 ? int(kAll) : it.step0 + int(per);
-            it.split = splits + of(sto - split) + t * c;
+            it.step0 = it.chunk * uniform(int(per));
+            it.step1 = c == 1 ? int(kAll) : it.step0 + uniform(int(per));
+            it.split = unsigned(uniform(int(splits))) + of(sto - split) + t * c;
             return it;
         }
         const auto last = [](unsigned v) { return unsigned(__builtin_amdgcn_readlane(int(v), kWave - 1)); };

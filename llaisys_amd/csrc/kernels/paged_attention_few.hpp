@@ -41,8 +41,8 @@ struct QueryRows {
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) f[t][h][e] = __builtin_amdgcn_ldexpf(f[t][h][e], exponent);
-                hi[t][h] = narrow8(f[t][h]);
-                if constexpr (kTwo) lo[t][h] = rest8(f[t][h], hi[t][h]);
+                if constexpr (kTwo) split8(f[t][h], hi[t][h], lo[t][h]);
+                else hi[t][h] = narrow8(f[t][h]);
             }
     }
 };
@@ -85,7 +85,7 @@ __global__ __launch_bounds__(kPagedThreads, NT <= 2 ? 2 : 1) void pagedFew(Paged
     q.load(a, m16 < rows, (size_t(it.start + token) * a.nh + size_t(head) * a.group + (row - token * a.group)) * dim, quarter);
     const float row_scale = __builtin_amdgcn_ldexpf(a.scale * kLog2e, 9 - q.exponent);
 
-    const int32_t *table = a.table + it.request * a.width;
+    const int32_t *table = a.table + int64_t(it.request) * a.width;
     const int in_block = (1 << a.shift) - 1;
     const size_t tile_bytes = size_t(dim) << a.shift;
 
@@ -179,8 +179,8 @@ __global__ __launch_bounds__(kPagedThreads, NT <= 2 ? 2 : 1) void pagedFew(Paged
                 l += x;
                 f[e] = some_hidden && t == -INFINITY ? 0.0f : x * w;
             }
-            p[u] = narrow8(f);
-            if constexpr (kTwoP) r[u] = rest8(f, p[u]);
+            if constexpr (kTwoP) split8(f, p[u], r[u]);
+            else p[u] = narrow8(f);
         }
         uint32_t v[16][NT];
 #pragma unroll

@@ -29,12 +29,14 @@ __device__ __forceinline__ int kColumn(int key, int piece) {
 }
 __device__ __forceinline__ int vColumn(int channel, int piece) { return piece ^ (((channel >> 2) & 7) ^ ((channel << 1) & 4)); }
 
+constexpr uint32_t kNone = 1, kZero = 2;
+
 template <int DP>
 struct Buffers {
     v4u k[2][kStep][DP / 8];   // [key][8 channels]
     v4u v[2][DP][kStep / 8];   // [channel][8 keys]
-    float ks[2][4], vs[2][4], lvs[2][4]; // of 16 keys: scales, and log2 of v's
-    int bad[2][4];             // their block id is none
+    v4f ks[2], vs[2], lvs[2];  // of 16 keys each: scales, and log2 of v's
+    v4u flags[2];              // kNone: their block id is none, kZero: their values are 0
 };
 template <int DP>
 struct ManyShared {
@@ -98,14 +100,14 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
             if (valid && 16 * s < dim) load8<T>(a.q, at + 16 * s, f); // again, from the cache: 8 values at a time in registers
 #pragma unroll
             for (int x = 0; x < 8; ++x) f[x] = __builtin_amdgcn_ldexpf(sign * f[x], e);
-            q[s] = narrow8(f);
-            if constexpr (kTwoQ) ql[s] = rest8(f, q[s]);
+            if constexpr (kTwoQ) split8(f, q[s], ql[s]);
+            else q[s] = narrow8(f);
         }
         row_scale = __builtin_amdgcn_ldexpf(fabsf(a.scale) * kLog2e, 9 - e);
     }
 
     // ---- the wave's 16 keys of a tile: HBM -> registers -> LDS
-    const int32_t *table = a.table + it.request * a.width;
+    const int32_t *table = a.table + int64_t(it.request) * a.width;
     const size_t tile_bytes = size_t(dim) << a.shift;
     const int in_block = (1 << a.shift) - 1;
     const int k_key = (lane * 16) / DP, k_piece = lane % (DP / 16); // i-th piece: key k_key + i * 1024 / DP
@@ -171,7 +173,7 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
             s.ks[b][wave] = checkedScale(ks);
             s.vs[b][wave] = v;
             s.lvs[b][wave] = __builtin_amdgcn_logf(v);
-            s.bad[b][wave] = bad;
+            s.flags[b][wave] = (bad ? kNone : 0) | (v == 0.0f ? kZero : 0);
         }
     };
 
@@ -184,53 +186,44 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
         for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
     const int my_key = 16 * (col / 4 % 2) + 4 * (col / 8) + col % 4; // K's row at this lane's place of the operand
 
-    const auto compute = [&](int step, int b) {
+    // kHide: some row of the wave does not see some key of the step
+    const auto compute = [&](auto hide_, int step, int b, bool zero) {
+        constexpr bool kHide = decltype(hide_)::value;
         const Buffers<DP> &s = sh.in;
+        // this lane's keys: 32 t + 16 half + 0..15
+        const v4f ks4 = s.ks[b], vs4 = s.vs[b], lvs4 = s.lvs[b];
+        const float kscale[2] = {half ? ks4.y : ks4.x, half ? ks4.w : ks4.z}, vscale[2] = {half ? vs4.y : vs4.x, half ? vs4.w : vs4.z};
+        const float lv[2] = {half ? lvs4.y : lvs4.x, half ? lvs4.w : lvs4.z};
         v16f sc[2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int i = 0; i < 16; ++i) sc[0][i] = sc[1][i] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sc[t][i] = 0.0f;
-            const int key = 32 * t + my_key;
+        for (int x = 0; x < kSteps; ++x)
 #pragma unroll
-            for (int x = 0; x < kSteps; ++x) {
+            for (int t = 0; t < 2; ++t) {
+                const int key = 32 * t + my_key;
                 const v8h k = __builtin_bit_cast(v8h, s.k[b][key][kColumn<DP>(key, 2 * x + half)]);
                 sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[x], sc[t], 0, 0, 0);
                 if constexpr (kTwoQ) sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[x], sc[t], 0, 0, 0);
             }
-        }
-        // this lane's keys: 32 t + 16 half + 0..15
-        float kscale[2], vscale[2], lv[2];
-        bool none[2], hide = (step + 1) * kStep > wave_first, zero = false;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            hide = hide || s.bad[b][g] != 0;
-            zero = zero || s.vs[b][g] == 0.0f;
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            kscale[t] = s.ks[b][2 * t + half];
-            vscale[t] = s.vs[b][2 * t + half];
-            lv[t] = s.lvs[b][2 * t + half];
-            none[t] = s.bad[b][2 * t + half] != 0;
-        }
-        hide = __builtin_amdgcn_readfirstlane(hide);
-        zero = __builtin_amdgcn_readfirstlane(zero);
         float c[2], top = -INFINITY, vtop = vref;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const int key0 = step * kStep + 32 * t + 16 * half;
             c[t] = row_scale * kscale[t];
-            if (hide) {
+            bool sees = true;
+            if constexpr (kHide) {
+                const bool none = (s.flags[b][2 * t + half] & kNone) != 0;
+                const int left = none ? 0 : limit - (step * kStep + 32 * t + 16 * half); // keys seen of the 16
+                sees = left > 0;
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (none[t] || key0 + i >= limit) sc[t][i] = -INFINITY;
+                    if (i >= left) sc[t][i] = -INFINITY;
             }
             float best = sc[t][0];
 #pragma unroll
             for (int i = 1; i < 16; ++i) best = fmaxf(best, sc[t][i]);
             top = fmaxf(top, best * c[t]);
-            vtop = hide && (none[t] || key0 >= limit) ? vtop : fmaxf(vtop, vscale[t]);
+            vtop = sees ? fmaxf(vtop, vscale[t]) : vtop;
         }
         top = butterflyStep<32, MaxOp>(top);
         vtop = butterflyStep<32, MaxOp>(vtop);
@@ -249,7 +242,7 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
         for (int t = 0; t < 2; ++t) {
             v8h p[2], r[2];
             float sum = 0.0f;
-            if (kTwoQ || zero || hide) {
+            if (kTwoQ || kHide || zero) {
                 const float w = vref > 0.0f ? vscale[t] / vref : vscale[t]; // 0, or NaN, where no scale was above 0
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
@@ -257,13 +250,13 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const float x = sc[t][8 * u + e];
-                        const bool out = hide && x == -INFINITY;
+                        const bool out = kHide && x == -INFINITY;
                         const float y = out ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(x, c[t], -base));
                         sum += y;
                         f[e] = out ? 0.0f : y * w;
                     }
-                    p[u] = narrow8(f);
-                    if constexpr (kTwoP) r[u] = rest8(f, p[u]);
+                    if constexpr (kTwoP) split8(f, p[u], r[u]);
+                    else p[u] = narrow8(f);
                 }
             } else {
                 // the value scale's ratio goes into the exponent, and out of the sum at once
@@ -276,8 +269,8 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
                         f[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][8 * u + e], c[t], -to));
                         sum += f[e];
                     }
-                    p[u] = narrow8(f);
-                    if constexpr (kTwoP) r[u] = rest8(f, p[u]);
+                    if constexpr (kTwoP) split8(f, p[u], r[u]);
+                    else p[u] = narrow8(f);
                 }
                 sum *= __builtin_amdgcn_exp2f(-shift);
             }
@@ -304,7 +297,14 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
         for (int step = it.step0, b = 0; step < end; ++step, b ^= 1) {
             if (step + 1 < end) stage(b ^ 1);
             if (step + 2 < end) fetch(step + 2);
-            if (step * kStep < wave_last) compute(step, b);
+            if (step * kStep < wave_last) {
+                const v4u f4 = sh.in.flags[b];
+                const uint32_t f = uint32_t(uniform(int(f4.x | f4.y | f4.z | f4.w)));
+                if ((step + 1) * kStep > wave_first || (f & kNone))
+                    compute(std::true_type{}, step, b, true);
+                else
+                    compute(std::false_type{}, step, b, (f & kZero) != 0);
+            }
             ldsBarrier();
         }
     }
