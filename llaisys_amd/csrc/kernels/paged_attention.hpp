@@ -295,15 +295,14 @@ __device__ __forceinline__ void mergePartials(const float *first, size_t stride,
     }
 }
 
-// Ends an item: `state(row, c, o, m, l)` gives 8 channels of the block's own result.  One chunk: the outputs.  Several: the
+// Ends an item: `state(row, c, o, m, l)` gives 8 channels of the block's own result, `place(row)` the row's first element in the output.  One chunk: the outputs.  Several: the
 // partial, and for the last of kFan chunks, and of those the last, the merge.
-template <typename T, int kTile, typename State>
-__device__ __forceinline__ void finishItem(const PagedAttnArgs &a, const Item &it, int head, int first_row, int rows, unsigned *shared,
-                                           State &&state) {
-    const int dim = a.dim, slots = dim / 8;
+template <typename T, int kTile, typename Place, typename State>
+__device__ __forceinline__ void finishItem(const PagedAttnArgs &a, const Item &it, int head, int rows, int dim, unsigned *shared,
+                                           Place &&place, State &&state) {
+    const int slots = dim / 8;
     const auto put = [&](int row, int c, const float *o, float, float l) {
-        const int m = first_row + row, i = m / a.group;
-        const size_t at = (size_t(it.start + i) * a.nh + size_t(head) * a.group + (m - i * a.group)) * dim + c;
+        const size_t at = place(row) + c;
         const float d = l == 0.0f ? 0.0f : 1.0f / l; // no key: 0
         float f[8];
 #pragma unroll

@@ -64,6 +64,7 @@ __global__ __launch_bounds__(kPagedThreads, NT <= 2 ? 2 : 1) void pagedFew(Paged
     constexpr int kRows = kFewTile, CH = 4 * NT, NW = kFewWaves;
     __shared__ struct {
         float m[NW][kRows], l[NW][kRows];
+        int at[kRows]; // a row's place in the output, from the tile's first token, in rows of dim
         float o[NW][kRows][64 * NT + 4];
     } sh;
     __shared__ unsigned arrived;
@@ -81,8 +82,10 @@ __global__ __launch_bounds__(kPagedThreads, NT <= 2 ? 2 : 1) void pagedFew(Paged
     if (!cutItem(it, steps)) return;
     const int end = min(it.step1, steps);
     const int limit = before + token + 1;
+    const int token0 = first_row / a.group, out_row = (token - token0) * a.nh + head * a.group + (row - token * a.group);
+    const size_t out0 = size_t(it.start + token0) * a.nh;
     QueryRows<T, NT> q;
-    q.load(a, m16 < rows, (size_t(it.start + token) * a.nh + size_t(head) * a.group + (row - token * a.group)) * dim, quarter);
+    q.load(a, m16 < rows, (out0 + unsigned(out_row)) * dim, quarter);
     const float row_scale = __builtin_amdgcn_ldexpf(a.scale * kLog2e, 9 - q.exponent);
 
     const int32_t *table = a.table + int64_t(it.request) * a.width;
@@ -235,6 +238,7 @@ __global__ __launch_bounds__(kPagedThreads, NT <= 2 ? 2 : 1) void pagedFew(Paged
     l = butterflyStep<16, SumOp>(l);
     l = butterflyStep<32, SumOp>(l);
     if (quarter == 0) {
+        if (wave == 0) sh.at[m16] = out_row;
         sh.m[wave][m16] = mx;
         sh.l[wave][m16] = l;
     }
@@ -246,7 +250,8 @@ __global__ __launch_bounds__(kPagedThreads, NT <= 2 ? 2 : 1) void pagedFew(Paged
             *reinterpret_cast<v4f *>(&sh.o[wave][m16][CH * (4 * quarter + i) + k]) =
                 v4f{acc[k][i] * unit, acc[k + 1][i] * unit, acc[k + 2][i] * unit, acc[k + 3][i] * unit};
     __syncthreads();
-    finishItem<T, kFewTile>(a, it, head, first_row, rows, &arrived, [&](int r, int c, float *o, float &m, float &sum) {
+    const auto place = [&](int r) { return (out0 + unsigned(sh.at[r])) * dim; };
+    finishItem<T, kFewTile>(a, it, head, rows, dim, &arrived, place, [&](int r, int c, float *o, float &m, float &sum) {
         m = -INFINITY;
         sum = 0.0f;
 #pragma unroll

@@ -18,7 +18,8 @@ static_assert(kManyTile == 32 * (kPagedThreads / kWave), "32 rows a wave");
 // Weights are 2^(t - m + 11): m stays while no score passes it by more than 2^4, so that few tiles rescale the sums.
 constexpr float kManyBits = 11.0f, kLazy = 4.0f;
 
-// Column of a 16-byte piece of a K row (key) and of a V row (channel) in LDS.
+// Column of a 16-byte piece of a K row (key) and of a V row (channel) in LDS.  xor distributes: the pieces 2 x + half of a key
+// lie at the place of piece `half`, xor 2 x.
 template <int DP>
 __device__ __forceinline__ int kColumn(int key, int piece) {
     // lanes of a read differ in bits 0, 1, 4, 2 of the key first
@@ -29,22 +30,17 @@ __device__ __forceinline__ int kColumn(int key, int piece) {
 }
 __device__ __forceinline__ int vColumn(int channel, int piece) { return piece ^ (((channel >> 2) & 7) ^ ((channel << 1) & 4)); }
 
-constexpr uint32_t kNone = 1, kZero = 2;
-
-template <int DP>
-struct Buffers {
-    v4u k[2][kStep][DP / 8];   // [key][8 channels]
-    v4u v[2][DP][kStep / 8];   // [channel][8 keys]
-    v4f ks[2], vs[2], lvs[2];  // of 16 keys each: scales, and log2 of v's
-    v4u flags[2];              // kNone: their block id is none, kZero: their values are 0
-};
+// Two buffers of each kind, a power of two apart: [key][channel] and [channel][key] f16, and for each 16 keys (scale of k,
+// of v, log2 of v's, whether their block id is none).  The outputs take their place.
 template <int DP>
 struct ManyShared {
+    static constexpr int kBuffer = kStep * DP * 2, kV = 2 * kBuffer, kScales = 4 * kBuffer;
     union {
-        Buffers<DP> in;
+        alignas(16) unsigned char in[4 * kBuffer + 128 + kWave * 16]; // the last: where lanes without a scale write theirs
         float out[kManyTile][DP + 4];
     };
     float m[kManyTile], l[kManyTile];
+    int at[kManyTile]; // a row's place in the output, from the tile's first token, in rows of dim
 };
 
 // Two blocks a compute unit where 256 registers hold a wave's rows.
@@ -58,7 +54,8 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
     constexpr int kSteps = DP / 16, kTiles = DP / 32;
     constexpr int kK = DP / 64;                 // 16-byte pieces of K a lane brings per tile
     constexpr int kV = DP <= 128 ? 1 : 2;       // units of 8 keys x 4 channels of V
-    __shared__ ManyShared<DP> sh;
+    using Sh = ManyShared<DP>;
+    __shared__ Sh sh;
     __shared__ unsigned arrived;
     const int dim = D ? D : a.dim;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave), lane = int(threadIdx.x) % kWave;
@@ -80,10 +77,12 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
     const bool valid = row < total_rows;
     const int limit = before + token + 1;
     const int wave_last = wrow < total_rows ? seenBy(min(wrow + 31, total_rows - 1)) : 0, wave_first = seenBy(wrow);
+    const int token0 = first_row / a.group, out_row = (token - token0) * a.nh + head * a.group + (row - token * a.group);
+    const size_t out0 = size_t(it.start + token0) * a.nh;
     v8h q[kSteps], ql[kTwoQ ? kSteps : 1];
     float row_scale;
     {
-        const size_t at = (size_t(it.start + token) * a.nh + size_t(head) * a.group + (row - token * a.group)) * dim + 8 * half;
+        const size_t at = (out0 + unsigned(out_row)) * dim + 8 * half;
         const float sign = a.scale < 0.0f ? -1.0f : 1.0f; // the scale of a score is not negative below
         float top = 0.0f;
 #pragma unroll
@@ -115,13 +114,14 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
     v4u kr[kK];
     uint32_t vr[kV][8];
     float ks = 0.0f, vs = 0.0f;
-    bool bad = false;
+    bool bad = false, any_bad = false;
     int id_next = 0;
+    // past the item's keys these read keys of its last block again
     const auto idOf = [&](int step) { return table[min(step * kStep + 16 * wave, seen_last - 1) >> a.shift]; };
     const auto fetch = [&](int step) { // uses id_next, and reads the id after it
-        const int id = __builtin_amdgcn_readfirstlane(id_next);
+        const int id = uniform(id_next);
         bad = uint32_t(id) >= uint32_t(a.n_blocks);
-        if (bad && lane == 0 && step * kStep + 16 * wave < seen_last) atomicOr(a.err, kErrPagedIndex);
+        any_bad = any_bad || (bad && step * kStep + 16 * wave < seen_last);
         const int64_t tile = (bad ? 0 : int64_t(id)) * a.heads + head;
         const size_t at = tile * tile_bytes + size_t((step * kStep + 16 * wave) & in_block) * dim;
         const int8_t *kp = a.k_codes + at, *vp = a.v_codes + at;
@@ -141,15 +141,22 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
         }
         ks = a.k_scale[tile];
         vs = a.v_scale[tile];
-        if (step + 1 < end) id_next = idOf(step + 1);
+        id_next = idOf(step + 1);
     };
-    const auto stage = [&](int b) {
-        Buffers<DP> &s = sh.in;
+    const auto put16 = [&](int at, const v8h &x) { *reinterpret_cast<v8h *>(sh.in + at) = x; };
+    const auto get16 = [&](int at) { return *reinterpret_cast<const v8h *>(sh.in + at); };
+    // places in the buffers, of the next step to write and the next to read
+    int k_to = (16 * wave + k_key) * DP * 2 + kColumn<DP>(16 * wave + k_key, 2 * k_piece) * 16;
+    int v_to = Sh::kV + 4 * v_quad * kStep * 2 + vColumn(4 * v_quad, 2 * wave + v_chunk) * 16;
+    int s_to = Sh::kScales + (lane == 0 ? wave * 16 : 128 + lane * 16);
+    const int s_flip = lane == 0 ? 64 : 0;
+    const auto stage = [&] {
 #pragma unroll
         for (int i = 0; i < kK; ++i) {
-            const int key = 16 * wave + k_key + i * (1024 / DP);
-            s.k[b][key][kColumn<DP>(key, 2 * k_piece)] = __builtin_bit_cast(v4u, codes8(kr[i].x, kr[i].y));
-            s.k[b][key][kColumn<DP>(key, 2 * k_piece + 1)] = __builtin_bit_cast(v4u, codes8(kr[i].z, kr[i].w));
+            // keys 1024 / DP apart: bit 2 of the key, where it changes, moves the column
+            const int at = k_to ^ (DP == 256 ? (i & 1) * 128 : 0);
+            put16(at + i * 2048, codes8(kr[i].x, kr[i].y));
+            put16((at ^ 16) + i * 2048, codes8(kr[i].z, kr[i].w));
         }
         if (DP >= 128 || lane < 32) {
 #pragma unroll
@@ -163,21 +170,19 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
                     Pairs p;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) p.p[e] = codePair(__builtin_amdgcn_perm(v[2 * e + 1], v[2 * e], kSel[x]));
-                    const int ch = 4 * v_quad + x;
-                    s.v[b][ch][vColumn(ch, 2 * wave + v_chunk + u)] = __builtin_bit_cast(v4u, join(p));
+                    put16((v_to ^ (u * 16) ^ (x / 2 * 64)) + x * kStep * 2, join(p));
                 }
             }
         }
-        if (lane == 0) {
-            const float v = checkedScale(vs);
-            s.ks[b][wave] = checkedScale(ks);
-            s.vs[b][wave] = v;
-            s.lvs[b][wave] = __builtin_amdgcn_logf(v);
-            s.flags[b][wave] = (bad ? kNone : 0) | (v == 0.0f ? kZero : 0);
-        }
+        const float v = checkedScale(vs);
+        *reinterpret_cast<v4u *>(sh.in + s_to) = v4u{__float_as_uint(checkedScale(ks)), __float_as_uint(v),
+                                                     __float_as_uint(__builtin_amdgcn_logf(v)), bad ? 1u : 0u};
+        k_to ^= Sh::kBuffer;
+        v_to ^= Sh::kBuffer;
+        s_to ^= s_flip;
     };
 
-    // ---- one tile's products
+    // ---- one step's products
     float mx = -INFINITY, l = 0.0f, vref = 0.0f, lref = 0.0f;
     v16f acc[kTiles];
 #pragma unroll
@@ -185,15 +190,13 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
     const int my_key = 16 * (col / 4 % 2) + 4 * (col / 8) + col % 4; // K's row at this lane's place of the operand
+    int k_from = my_key * DP * 2 + kColumn<DP>(my_key, half) * 16;
+    int v_from = Sh::kV + col * kStep * 2 + vColumn(col, 2 * half) * 16;
+    int s_from = Sh::kScales;
 
-    // kHide: some row of the wave does not see some key of the step
-    const auto compute = [&](auto hide_, int step, int b, bool zero) {
-        constexpr bool kHide = decltype(hide_)::value;
-        const Buffers<DP> &s = sh.in;
-        // this lane's keys: 32 t + 16 half + 0..15
-        const v4f ks4 = s.ks[b], vs4 = s.vs[b], lvs4 = s.lvs[b];
-        const float kscale[2] = {half ? ks4.y : ks4.x, half ? ks4.w : ks4.z}, vscale[2] = {half ? vs4.y : vs4.x, half ? vs4.w : vs4.z};
-        const float lv[2] = {half ? lvs4.y : lvs4.x, half ? lvs4.w : lvs4.z};
+    // The next step's codes are staged beside the first product, those of the one after it asked for.  `hide`: some row of
+    // the wave does not see some key of the step.
+    const auto compute = [&](int step, const v4u (&info)[4], bool hide) {
         v16f sc[2];
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[0][i] = sc[1][i] = 0.0f;
@@ -201,29 +204,54 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
         for (int x = 0; x < kSteps; ++x)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const int key = 32 * t + my_key;
-                const v8h k = __builtin_bit_cast(v8h, s.k[b][key][kColumn<DP>(key, 2 * x + half)]);
+                const v8h k = get16((k_from ^ (x * 32)) + t * 32 * DP * 2);
                 sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[x], sc[t], 0, 0, 0);
                 if constexpr (kTwoQ) sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[x], sc[t], 0, 0, 0);
             }
-        float c[2], top = -INFINITY, vtop = vref;
+        stage();
+        fetch(step + 2);
+        if constexpr (!kTwoQ) {
+            // a few operands ahead, the conversions between the products
+            constexpr int kAhead = 4;
+            __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0); // LDS reads
+#pragma unroll
+            for (int i = 0; i < 2 * kSteps; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); // MFMA
+                if (i < 2 * kSteps - kAhead) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 6, 0); // VALU
+            }
+        }
+        // this lane's keys: 32 t + 16 half + 0..15
+        float c[2], vscale[2], shift[2];
+        bool sees[2] = {true, true};
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            c[t] = row_scale * kscale[t];
-            bool sees = true;
-            if constexpr (kHide) {
-                const bool none = (s.flags[b][2 * t + half] & kNone) != 0;
+            c[t] = row_scale * __uint_as_float(half ? info[2 * t + 1].x : info[2 * t].x);
+            vscale[t] = __uint_as_float(half ? info[2 * t + 1].y : info[2 * t].y);
+            shift[t] = __uint_as_float(half ? info[2 * t + 1].z : info[2 * t].z);
+        }
+        if (hide) {
+            // a hidden key's score is so low that its weight is 0 for any factor from 1e-30 on; a smaller factor makes every
+            // score 0 as 1e-30 does, and where no key of the 16 is seen neither scale may speak (they may be NaN)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const bool none = (half ? info[2 * t + 1].w : info[2 * t].w) != 0;
                 const int left = none ? 0 : limit - (step * kStep + 32 * t + 16 * half); // keys seen of the 16
-                sees = left > 0;
+                sees[t] = left > 0;
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (i >= left) sc[t][i] = -INFINITY;
+                    if (i >= left) sc[t][i] = -3e38f;
+                if (c[t] < 1e-30f || !sees[t]) c[t] = 1e-30f;
             }
+        }
+        float top = -INFINITY, vtop = vref;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
             float best = sc[t][0];
 #pragma unroll
             for (int i = 1; i < 16; ++i) best = fmaxf(best, sc[t][i]);
-            top = fmaxf(top, best * c[t]);
-            vtop = sees ? fmaxf(vtop, vscale[t]) : vtop;
+            top = sees[t] ? fmaxf(top, best * c[t]) : top;
+            vtop = sees[t] ? fmaxf(vtop, vscale[t]) : vtop;
         }
         top = butterflyStep<32, MaxOp>(top);
         vtop = butterflyStep<32, MaxOp>(vtop);
@@ -241,72 +269,64 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             v8h p[2], r[2];
-            float sum = 0.0f;
-            if (kTwoQ || kHide || zero) {
-                const float w = vref > 0.0f ? vscale[t] / vref : vscale[t]; // 0, or NaN, where no scale was above 0
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    float f[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float x = sc[t][8 * u + e];
-                        const bool out = kHide && x == -INFINITY;
-                        const float y = out ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(x, c[t], -base));
-                        sum += y;
-                        f[e] = out ? 0.0f : y * w;
-                    }
-                    if constexpr (kTwoP) split8(f, p[u], r[u]);
-                    else p[u] = narrow8(f);
-                }
+            float sum = 0.0f, to = base, w = 1.0f;
+            if constexpr (kTwoQ) {
+                w = !sees[t] ? 0.0f : vref > 0.0f ? vscale[t] / vref : vscale[t]; // 0, or NaN, where no scale was above 0
             } else {
-                // the value scale's ratio goes into the exponent, and out of the sum at once
-                const float shift = lv[t] - lref, to = base - shift;
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    float f[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        f[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][8 * u + e], c[t], -to));
-                        sum += f[e];
-                    }
-                    if constexpr (kTwoP) split8(f, p[u], r[u]);
-                    else p[u] = narrow8(f);
-                }
-                sum *= __builtin_amdgcn_exp2f(-shift);
+                // the value scale's ratio goes into the exponent, and out of the sum at once; below 2^-100 (or 0) the
+                // weights are 0 as f16
+                const float d = shift[t] - lref;
+                shift[t] = !sees[t] ? 0.0f : d < -100.0f ? -100.0f : d;
+                to = base - shift[t];
             }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float f[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    f[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][8 * u + e], c[t], -to));
+                    sum += f[e];
+                    if constexpr (kTwoQ) f[e] *= w;
+                }
+                if constexpr (kTwoP) split8(f, p[u], r[u]);
+                else p[u] = narrow8(f);
+            }
+            if constexpr (!kTwoQ) sum *= __builtin_amdgcn_exp2f(-shift[t]);
             l += sum;
 #pragma unroll
-            for (int k = 0; k < kTiles; ++k) {
-                const int ch = 32 * k + col;
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const v8h v = __builtin_bit_cast(v8h, s.v[b][ch][vColumn(ch, 4 * t + 2 * half + u)]);
+                for (int k = 0; k < kTiles; ++k) {
+                    const v8h v = get16((v_from ^ ((4 * t + u) * 16)) + k * 32 * kStep * 2);
                     acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[u], acc[k], 0, 0, 0);
                     if constexpr (kTwoP) acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, r[u], acc[k], 0, 0, 0);
                 }
-            }
         }
     };
 
     if (it.step0 < end) {
         id_next = idOf(it.step0);
         fetch(it.step0);
-        stage(0);
-        if (it.step0 + 1 < end) fetch(it.step0 + 1);
+        stage();
+        fetch(it.step0 + 1);
         ldsBarrier();
-        for (int step = it.step0, b = 0; step < end; ++step, b ^= 1) {
-            if (step + 1 < end) stage(b ^ 1);
-            if (step + 2 < end) fetch(step + 2);
+        for (int step = it.step0; step < end; ++step) {
             if (step * kStep < wave_last) {
-                const v4u f4 = sh.in.flags[b];
-                const uint32_t f = uint32_t(uniform(int(f4.x | f4.y | f4.z | f4.w)));
-                if ((step + 1) * kStep > wave_first || (f & kNone))
-                    compute(std::true_type{}, step, b, true);
-                else
-                    compute(std::false_type{}, step, b, (f & kZero) != 0);
+                v4u info[4];
+#pragma unroll
+                for (int g = 0; g < 4; ++g) info[g] = *reinterpret_cast<const v4u *>(sh.in + s_from + 16 * g);
+                const bool none = uniform(int(info[0].w | info[1].w | info[2].w | info[3].w)) != 0;
+                compute(step, info, none || (step + 1) * kStep > wave_first);
+            } else {
+                stage();
+                fetch(step + 2);
             }
+            k_from ^= Sh::kBuffer;
+            v_from ^= Sh::kBuffer;
+            s_from ^= 64;
             ldsBarrier();
         }
+        if (any_bad && lane == 0) atomicOr(a.err, kErrPagedIndex);
     }
 
     // ---- outputs through LDS: row, 8 channels
@@ -323,14 +343,17 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
     if (half == 0) {
         sh.m[mine] = mx;
         sh.l[mine] = l;
+        sh.at[mine] = out_row;
     }
     __syncthreads();
-    finishItem<T, kManyTile>(a, it, head, first_row, rows, &arrived, [&](int r, int c, float *o, float &m, float &sum) {
-        m = sh.m[r];
-        sum = sh.l[r];
+    finishItem<T, kManyTile>(
+        a, it, head, rows, dim, &arrived, [&](int r) { return (out0 + unsigned(sh.at[r])) * dim; },
+        [&](int r, int c, float *o, float &m, float &sum) {
+            m = sh.m[r];
+            sum = sh.l[r];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = sh.out[r][c + e];
-    });
+            for (int e = 0; e < 8; ++e) o[e] = sh.out[r][c + e];
+        });
 }
 
 template <typename T>
