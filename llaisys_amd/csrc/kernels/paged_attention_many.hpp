@@ -150,36 +150,41 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
     int v_to = Sh::kV + 4 * v_quad * kStep * 2 + vColumn(4 * v_quad, 2 * wave + v_chunk) * 16;
     int s_to = Sh::kScales + (lane == 0 ? wave * 16 : 128 + lane * 16);
     const int s_flip = lane == 0 ? 64 : 0;
-    const auto stage = [&] {
-#pragma unroll
-        for (int i = 0; i < kK; ++i) {
+    // The staging in pieces, to be put between products: 2 kK of K, 4 kV of V.
+    constexpr int kPieces = 2 * kK + 4 * kV;
+    uint32_t vx[kV][8];
+    const auto stagePiece = [&](int j) {
+        if (j < 2 * kK) {
             // keys 1024 / DP apart: bit 2 of the key, where it changes, moves the column
-            const int at = k_to ^ (DP == 256 ? (i & 1) * 128 : 0);
-            put16(at + i * 2048, codes8(kr[i].x, kr[i].y));
-            put16((at ^ 16) + i * 2048, codes8(kr[i].z, kr[i].w));
+            const int i = j / 2, at = k_to ^ (DP == 256 ? (i & 1) * 128 : 0) ^ (j % 2 * 16);
+            put16(at + i * 2048, j % 2 ? codes8(kr[i].z, kr[i].w) : codes8(kr[i].x, kr[i].y));
+            return;
         }
-        if (DP >= 128 || lane < 32) {
+        const int u = (j - 2 * kK) / 4, x = (j - 2 * kK) % 4;
+        constexpr uint32_t kSel[4] = {0x0c040c00u, 0x0c050c01u, 0x0c060c02u, 0x0c070c03u};
+        if (x == 0) {
 #pragma unroll
-            for (int u = 0; u < kV; ++u) {
-                uint32_t v[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = vr[u][i] ^ 0x80808080u;
-                constexpr uint32_t kSel[4] = {0x0c040c00u, 0x0c050c01u, 0x0c060c02u, 0x0c070c03u};
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    Pairs p;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) p.p[e] = codePair(__builtin_amdgcn_perm(v[2 * e + 1], v[2 * e], kSel[x]));
-                    put16((v_to ^ (u * 16) ^ (x / 2 * 64)) + x * kStep * 2, join(p));
-                }
-            }
+            for (int i = 0; i < 8; ++i) vx[u][i] = vr[u][i] ^ 0x80808080u;
         }
+        Pairs p;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p.p[e] = codePair(__builtin_amdgcn_perm(vx[u][2 * e + 1], vx[u][2 * e], kSel[x]));
+        // (of 64 channels half the lanes have none: theirs go behind the scales)
+        const int at = (v_to ^ (u * 16) ^ (x / 2 * 64)) + x * kStep * 2;
+        put16(DP >= 128 || lane < 32 ? at : Sh::kScales + 128 + lane * 16, join(p));
+    };
+    const auto stageScales = [&] {
         const float v = checkedScale(vs);
         *reinterpret_cast<v4u *>(sh.in + s_to) = v4u{__float_as_uint(checkedScale(ks)), __float_as_uint(v),
                                                      __float_as_uint(__builtin_amdgcn_logf(v)), bad ? 1u : 0u};
         k_to ^= Sh::kBuffer;
         v_to ^= Sh::kBuffer;
         s_to ^= s_flip;
+    };
+    const auto stage = [&] {
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) stagePiece(j);
+        stageScales();
     };
 
     // ---- one step's products
@@ -200,27 +205,29 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
         v16f sc[2];
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[0][i] = sc[1][i] = 0.0f;
+        // operands two products ahead, a piece of the staging before each product
+        v8h k[3][2];
+        const auto readK = [&](int x) {
 #pragma unroll
-        for (int x = 0; x < kSteps; ++x)
+            for (int t = 0; t < 2; ++t) k[x % 3][t] = get16((k_from ^ (x * 32)) + t * 32 * DP * 2);
+        };
+        readK(0);
+        if constexpr (kSteps > 1) readK(1);
+#pragma unroll
+        for (int x = 0; x < kSteps; ++x) {
+            if (x + 2 < kSteps) readK(x + 2);
+#pragma unroll
+            for (int j = x * kPieces / kSteps; j < (x + 1) * kPieces / kSteps; ++j) stagePiece(j);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const v8h k = get16((k_from ^ (x * 32)) + t * 32 * DP * 2);
-                sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[x], sc[t], 0, 0, 0);
-                if constexpr (kTwoQ) sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[x], sc[t], 0, 0, 0);
+                sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[x % 3][t], q[x], sc[t], 0, 0, 0);
+                if constexpr (kTwoQ) sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[x % 3][t], ql[x], sc[t], 0, 0, 0);
             }
-        stage();
-        fetch(step + 2);
-        if constexpr (!kTwoQ) {
-            // a few operands ahead, the conversions between the products
-            constexpr int kAhead = 4;
-            __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0); // LDS reads
-#pragma unroll
-            for (int i = 0; i < 2 * kSteps; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); // MFMA
-                if (i < 2 * kSteps - kAhead) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x002, 6, 0); // VALU
-            }
+            __builtin_amdgcn_sched_barrier(0);
         }
+        stageScales();
+        fetch(step + 2);
         // this lane's keys: 32 t + 16 half + 0..15
         float c[2], vscale[2], shift[2];
         bool sees[2] = {true, true};
@@ -266,41 +273,57 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
             lref = vref > 0.0f ? __builtin_amdgcn_logf(vref) : 0.0f;
         }
         const float base = (mx == -INFINITY ? 0.0f : mx) - kManyBits;
+        float to[2], w[2], sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            v8h p[2], r[2];
-            float sum = 0.0f, to = base, w = 1.0f;
+            to[t] = base;
             if constexpr (kTwoQ) {
-                w = !sees[t] ? 0.0f : vref > 0.0f ? vscale[t] / vref : vscale[t]; // 0, or NaN, where no scale was above 0
+                w[t] = !sees[t] ? 0.0f : vref > 0.0f ? vscale[t] / vref : vscale[t]; // 0, or NaN, where no scale was above 0
             } else {
                 // the value scale's ratio goes into the exponent, and out of the sum at once; below 2^-100 (or 0) the
                 // weights are 0 as f16
                 const float d = shift[t] - lref;
                 shift[t] = !sees[t] ? 0.0f : d < -100.0f ? -100.0f : d;
-                to = base - shift[t];
+                to[t] = base - shift[t];
             }
+        }
+        // eight weights at a time, those of the next eight keys computed between the products of these
+        float f[2][8];
+        v8h v[2][kTiles];
+        const auto weight = [&](int g, int e) {
+            const int t = g / 2;
+            float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][8 * (g % 2) + e], c[t], -to[t]));
+            sum[t] += x;
+            if constexpr (kTwoQ) x *= w[t];
+            f[g % 2][e] = x;
+        };
+        const auto readV = [&](int g, int k) { v[g % 2][k] = get16((v_from ^ ((g / 2 * 4 + g % 2) * 16)) + k * 32 * kStep * 2); };
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                float f[8];
+        for (int k = 0; k < kTiles; ++k) readV(0, k);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    f[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][8 * u + e], c[t], -to));
-                    sum += f[e];
-                    if constexpr (kTwoQ) f[e] *= w;
+        for (int e = 0; e < 8; ++e) weight(0, e);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            v8h p, r;
+            if constexpr (kTwoP) split8(f[g % 2], p, r);
+            else p = narrow8(f[g % 2]);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < kTiles; ++k) {
+                acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[g % 2][k], p, acc[k], 0, 0, 0);
+                if constexpr (kTwoP) acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[g % 2][k], r, acc[k], 0, 0, 0);
+                if (g < 3) {
+                    readV(g + 1, k);
+#pragma unroll
+                    for (int e = k * 8 / kTiles; e < (k + 1) * 8 / kTiles; ++e) weight(g + 1, e);
                 }
-                if constexpr (kTwoP) split8(f, p[u], r[u]);
-                else p[u] = narrow8(f);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            if constexpr (!kTwoQ) sum *= __builtin_amdgcn_exp2f(-shift[t]);
-            l += sum;
+        }
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int k = 0; k < kTiles; ++k) {
-                    const v8h v = get16((v_from ^ ((4 * t + u) * 16)) + k * 32 * kStep * 2);
-                    acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[u], acc[k], 0, 0, 0);
-                    if constexpr (kTwoP) acc[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, r[u], acc[k], 0, 0, 0);
-                }
+        for (int t = 0; t < 2; ++t) {
+            if constexpr (!kTwoQ) sum[t] *= __builtin_amdgcn_exp2f(-shift[t]);
+            l += sum[t];
         }
     };
 
