@@ -17,7 +17,7 @@ constexpr unsigned kTarget = 512; // chunks over all heads: two blocks on each o
 
 // What the sizes known to the host allow: the requests' lengths are on the device.
 struct Plan {
-    size_t items;  // per head, at most
+    size_t items;  // of each head, at most
     size_t splits; // partials
     unsigned target;
 };

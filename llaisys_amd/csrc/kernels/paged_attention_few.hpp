@@ -70,8 +70,8 @@ __global__ __launch_bounds__(kPagedThreads, NT <= 2 ? 2 : 1) void pagedFew(Paged
     __shared__ unsigned arrived;
     const int dim = D ? D : a.dim;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave), lane = int(threadIdx.x) % kWave;
-    const int m16 = lane % 16, quarter = lane / 16, head = int(blockIdx.y);
-    Item it = findItem<kRows>(a, blockIdx.x, blockIdx.x == 0 && head == 0 && wave == 0);
+    const int m16 = lane % 16, quarter = lane / 16, head = int(blockIdx.x % unsigned(a.heads));
+    Item it = findItem<kRows>(a, blockIdx.x / unsigned(a.heads), blockIdx.x == 0 && wave == 0);
     if (!it.any) return;
 
     const int first_row = it.tile * kRows, rows = min(kRows, it.n * a.group - first_row);
@@ -270,7 +270,7 @@ __global__ __launch_bounds__(kPagedThreads, NT <= 2 ? 2 : 1) void pagedFew(Paged
 
 template <typename T>
 void launchPagedFew(const PagedAttnArgs &a, unsigned items, hipStream_t s) {
-    const dim3 grid(items, unsigned(a.heads));
+    const unsigned grid = items * unsigned(a.heads);
     if (a.dim == 128) pagedFew<T, 2, 128><<<grid, kPagedThreads, 0, s>>>(a);
     else if (a.dim == 64) pagedFew<T, 1, 64><<<grid, kPagedThreads, 0, s>>>(a);
     else if (a.dim < 64) pagedFew<T, 1, 0><<<grid, kPagedThreads, 0, s>>>(a);

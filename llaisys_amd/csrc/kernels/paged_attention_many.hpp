@@ -59,8 +59,8 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
     __shared__ unsigned arrived;
     const int dim = D ? D : a.dim;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave), lane = int(threadIdx.x) % kWave;
-    const int col = lane % 32, half = lane / 32, head = int(blockIdx.y);
-    Item it = findItem<kManyTile>(a, blockIdx.x, blockIdx.x == 0 && head == 0 && wave == 0);
+    const int col = lane % 32, half = lane / 32, head = int(blockIdx.x % unsigned(a.heads));
+    Item it = findItem<kManyTile>(a, blockIdx.x / unsigned(a.heads), blockIdx.x == 0 && wave == 0);
     if (!it.any) return;
 
     const int total_rows = it.n * a.group;
@@ -381,7 +381,7 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
 
 template <typename T>
 void launchPagedMany(const PagedAttnArgs &a, unsigned items, hipStream_t s) {
-    const dim3 grid(items, unsigned(a.heads));
+    const unsigned grid = items * unsigned(a.heads);
     if (a.dim == 128) pagedMany<T, 128, 128><<<grid, kPagedThreads, 0, s>>>(a);
     else if (a.dim == 64) pagedMany<T, 64, 64><<<grid, kPagedThreads, 0, s>>>(a);
     else if (a.dim < 64) pagedMany<T, 64, 0><<<grid, kPagedThreads, 0, s>>>(a);

@@ -159,7 +159,9 @@ void pagedAttentionInt8KV(tensor_t attn_val, tensor_t q, tensor_t k_cache, tenso
     ASSERT(kv_lens->numel() == requests && row_starts->numel() == requests + 1,
            "PagedAttentionInt8KV: kv_lens must hold a length per request and row_starts requests + 1 elements");
     ASSERT(rows < kLimit && requests < kLimit && nh <= 65535, "PagedAttentionInt8KV: sizes must be below 2^31, heads at most 65535");
-    ASSERT(rows * (nh / c.heads) < kLimit, "PagedAttentionInt8KV: rows times q heads of a kv head must be below 2^31");
+    // one launch: fewer than 2^24 blocks of 256 threads, 16 rows of a kv head each at the least
+    ASSERT(rows * nh / 16 + requests * c.heads < (size_t(1) << 24) - (size_t(1) << 17),
+           "PagedAttentionInt8KV: too many rows and heads for one call");
     ASSERT(width < kLimit && width * c.block <= kLimit - 4096, "PagedAttentionInt8KV: a request's blocks must hold fewer than 2^31 tokens");
     ASSERT(!overlaps(attn_val, q), "PagedAttentionInt8KV: attn_val must not overlap q");
     requireAligned(q, op);
