@@ -49,6 +49,7 @@ template <typename T>
 void launch(PagedAttnArgs a, const PagedAttentionCall &c, bool split, hipStream_t s) {
     const auto with = [&](const Plan &p, int least, int most) {
         a.target = split ? p.target : 0;
+        a.per_target = 1.0f / float(kTarget);
         a.few_most = most;
         a.many_least = least;
         return a;
@@ -74,9 +75,9 @@ void pagedAttentionInt8KV(const PagedAttentionCall &c, void *ws, size_t ws_bytes
     char *head = static_cast<char *>(ws);
     const PagedAttnArgs a{c.out, c.q, c.cache.k_codes, c.cache.v_codes, c.cache.k_scale, c.cache.v_scale, c.table, c.starts, c.lens,
                           reinterpret_cast<float *>(head + kScratchReserved), reinterpret_cast<unsigned *>(head + kPagedCountersOffset),
-                          0, 0, INT_MAX, int64_t(c.rows), int64_t(c.requests), int64_t(c.width),
+                          0, 0.0f, 0, INT_MAX, int64_t(c.rows), int64_t(c.requests), int64_t(c.width),
                           int64_t(c.cache.n_blocks), int(c.nh), int(c.cache.heads), int(c.nh / c.cache.heads), int(c.cache.dim),
-                          __builtin_ctzll(c.cache.block), c.scale, c.err};
+                          __builtin_ctzll(c.cache.block), SmallDiv(uint32_t(c.cache.heads)), SmallDiv(uint32_t(c.nh / c.cache.heads)), c.scale, c.err};
     switch (c.dt) {
     case LLAISYS_DTYPE_F32: return launch<F32>(a, c, split, s);
     case LLAISYS_DTYPE_BF16: return launch<BF16>(a, c, split, s);

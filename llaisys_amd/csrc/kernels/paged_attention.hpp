@@ -7,9 +7,9 @@
 // are split into chunks of a whole number of steps, and whoever finishes a tile's last chunk merges them.
 //
 // Codes meet the matrix instructions as f16: a code is a whole number of magnitude <= 127, exact in f16, for
-// every element type of q.  Rows of q are multiplied by a power of two that brings their largest element to
-// [2^14, 2^15): bf16 and f16 rows then are exact f16 (but for elements below 2^-38 of the row's largest), f32 rows
-// enter as two f16 parts (22 bits).  Weights p = 2^(t - m) lie in [0, 1], enter times 2^15 (f16's normal range
+// every element type of q.  f16 rows of q enter as they are; others are multiplied by a power of two that brings their
+// largest element to [2^14, 2^15): bf16 rows then are exact f16 (but for elements below 2^-38 of the row's largest), f32
+// rows enter as two f16 parts (22 bits).  Weights p = 2^(t - m) lie in [0, 1], enter times 2^15 (f16's normal range
 // then goes down to 2^-29), and in two parts where the rows are f16 or f32; bf16 rows round the result to 8 bits, 11 for
 // a weight are enough.  A block's scale of v multiplies the weights as its ratio to the largest seen so
 // far, so that nothing leaves f16's range.
@@ -17,6 +17,9 @@
 
 #include "common.hpp"
 #include "launch.hpp"
+#include "quantize.hpp"
+
+#include <type_traits>
 
 namespace llaisys::kernels {
 
@@ -30,6 +33,20 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kCodeUnit = 0x1p-9f; // a code's f16 value is code * kCodeUnit
 constexpr float kWeightBits = 15.0f; // weights are 2^(t - m + kWeightBits)
 
+// Division of n < 2^31 by a launch constant d < 2^16.  With 2^s < d <= 2^(s + 1) and m = ceil(2^(32 + s) / d) < 2^32,
+// n m / 2^(32 + s) is above n / d by n (m d - 2^(32 + s)) / (d 2^(32 + s)) < 2^31 2^(s + 1) / (d 2^(32 + s)) = 1 / d, so its
+// whole part is that of n / d.
+struct SmallDiv {
+    uint32_t m = 0, s = 0; // m 0: d is 1
+    SmallDiv() = default;
+    explicit SmallDiv(uint32_t d) {
+        if (d <= 1) return;
+        while ((2u << s) < d) ++s;
+        m = uint32_t(((uint64_t(1) << (32 + s)) + d - 1) / d);
+    }
+    __device__ __forceinline__ int div(int n) const { return m ? int(__umulhi(uint32_t(n), m) >> s) : n; }
+};
+
 struct PagedAttnArgs {
     void *out;
     const void *q;
@@ -39,9 +56,11 @@ struct PagedAttnArgs {
     float *part;        // partials of chunks of split tiles
     unsigned *arrived;  // [2][kPagedCounters], 0 between launches
     unsigned target;    // chunks wanted over all requests and heads; 0: no tile is split
+    float per_target;   // 1 / target
     int few_most, many_least; // rows of the requests that the launch attends: up to, from
     int64_t rows, requests, width, n_blocks;
     int nh, heads, group, dim, shift;
+    SmallDiv by_heads, by_group;
     float scale;
     int *err;
 };
@@ -91,10 +110,41 @@ __device__ __forceinline__ void split8(const float *f, v8h &hi, v8h &lo) {
     for (int e = 0; e < 8; ++e) lo[e] = _Float16(f[e] - float(hi[e]));
 }
 
+// Eight elements of a row as loaded, as values, and the largest finite magnitude over some of them.
 template <typename T>
-__device__ __forceinline__ void load8(const void *base, size_t elem, float *f) {
-    Fmt<T>::unpack(load16<T>(base, elem), f);
-    if constexpr (Fmt<T>::kVec == 4) Fmt<T>::unpack(load16<T>(base, elem + 4), f + 4);
+struct Raw8 {
+    static constexpr int kN = 8 / Fmt<T>::kVec;
+    v4u r[kN];
+    __device__ __forceinline__ void load(const void *base, size_t elem) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) r[i] = load16<T>(base, elem + i * Fmt<T>::kVec);
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) r[i] = v4u{0, 0, 0, 0};
+    }
+    __device__ __forceinline__ void unpack(float *f) const {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) Fmt<T>::unpack(r[i], f + i * Fmt<T>::kVec);
+    }
+};
+template <typename T, int N>
+__device__ __forceinline__ float largest(const Raw8<T> (&x)[N]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int s = 0; s < N; ++s)
+#pragma unroll
+        for (int i = 0; i < Raw8<T>::kN; ++i) m = AbsBits<T>::fold(m, x[s].r[i]);
+    m = AbsBits<T>::finish(m);
+    if (__builtin_expect(m < AbsBits<T>::kInf, 1)) return AbsBits<T>::value(m);
+    float top = 0.0f;
+    for (int s = 0; s < N; ++s) {
+        float f[8];
+        x[s].unpack(f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fabsf(f[e]) < INFINITY && fabsf(f[e]) > top ? fabsf(f[e]) : top;
+    }
+    return top;
 }
 
 // Eight outputs, rounded once, to nearest (f16 by the conversion instruction).
@@ -110,19 +160,24 @@ __device__ __forceinline__ void store8(void *base, size_t elem, const float *f) 
     }
 }
 
-// Largest finite magnitude of f's elements so far.
-__device__ __forceinline__ float foldFinite(float m, const float *f) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float x = fabsf(f[e]);
-        m = x < INFINITY && x > m ? x : m;
-    }
-    return m;
-}
 // Exponent that brings `top` to [2^14, 2^15).
 __device__ __forceinline__ int rowExponent(float top) { return top > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0; }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Inclusive sums over the wave's lanes, without LDS: shifts within rows of 16 lanes, then of the rows' last lanes.
+__device__ __forceinline__ unsigned waveScan(unsigned v) {
+    const auto add = [](unsigned x, auto ctrl, auto rows, auto banks) {
+        return x + unsigned(__builtin_amdgcn_update_dpp(0, int(x), decltype(ctrl)::value, decltype(rows)::value, decltype(banks)::value, false));
+    };
+    using std::integral_constant;
+    v = add(v, integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{}, integral_constant<int, 0xF>{}); // row_shr:1
+    v = add(v, integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{}, integral_constant<int, 0xF>{}); // row_shr:2
+    v = add(v, integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{}, integral_constant<int, 0xE>{}); // row_shr:4
+    v = add(v, integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{}, integral_constant<int, 0xC>{}); // row_shr:8
+    v = add(v, integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{}, integral_constant<int, 0xF>{}); // row_bcast:15
+    return add(v, integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{}, integral_constant<int, 0xF>{}); // row_bcast:31
+}
 
 // What a block of threads works at: a tile of one request's rows and a chunk of its keys.
 struct Item {
@@ -144,78 +199,76 @@ struct Item {
 // The item of index `index`: requests in order, of each its tiles, of each its chunks.  Every wave finds it by
 // itself: sums over the requests 64 at a time, so that no table of items has to be made before.
 template <int kTile>
-__device__ __forceinline__ Item findItem(const PagedAttnArgs &a, unsigned index, bool report) {
+__device__ __forceinline__ Item findItem(const PagedAttnArgs &a, int index, bool report) {
     const int lane = threadIdx.x % kWave;
-    const auto request = [&](int64_t r, int &start, int &n, int &len) { // false: out of range, skipped
-        start = n = len = 0;
+    struct Request {
+        int start, n, len;
+    };
+    const auto request = [&](int64_t r, Request &q) { // false: out of range, skipped
+        q = Request{0, 0, 0};
         if (r >= a.requests) return true;
-        const int64_t s0 = a.starts[r], s1 = a.starts[r + 1], k = a.lens[r];
+        const int s0 = a.starts[r], s1 = a.starts[r + 1], k = a.lens[r];
         if (s0 < 0 || s1 < s0 || s1 > a.rows || k < 0 || k > (a.width << a.shift)) return false;
-        const int rows = int(s1 - s0) * a.group;
-        if (rows > a.few_most || rows < a.many_least) return true; // another launch's
-        start = int(s0);
-        n = int(s1 - s0);
-        len = int(k);
+        const int rows = (s1 - s0) * a.group;
+        if (rows <= a.few_most && rows >= a.many_least) q = Request{s0, s1 - s0, k}; // (else another launch's)
         return true;
     };
-    const auto tilesOf = [&](int n) { return (unsigned(n * a.group) + kTile - 1) / kTile; };
-    const auto stepsOf = [&](int len) { return (unsigned(len) + kStep - 1) / kStep; };
+    const auto tilesOf = [&](const Request &q) { return (unsigned(q.n * a.group) + kTile - 1) / kTile; };
+    const auto stepsOf = [&](const Request &q) { return (unsigned(q.len) + kStep - 1) / kStep; };
     constexpr unsigned kAll = 0x7FFFFFFFu;
     unsigned per = kAll; // steps of a chunk
-    int start, n, len;
+    Request q, first;
+    bool fine = request(lane, first);
     if (a.target || report) {
-        uint64_t total = 0;
-        bool fine = true;
-        for (int64_t r0 = 0; r0 < a.requests; r0 += kWave) {
-            fine = request(r0 + lane, start, n, len) && fine;
-            total += uint64_t(tilesOf(n)) * stepsOf(len);
+        // (in f32: the sum decides how far keys are split, and is rounded up by more than it can be off)
+        float total = float(tilesOf(first)) * float(stepsOf(first));
+        for (int64_t r0 = kWave; r0 < a.requests; r0 += kWave) {
+            fine = request(r0 + lane, q) && fine;
+            total += float(tilesOf(q)) * float(stepsOf(q));
         }
-#pragma unroll
-        for (int m = 1; m < kWave; m <<= 1) total += (uint64_t(uint32_t(__shfl_xor(int(total >> 32), m, kWave))) << 32) | uint32_t(__shfl_xor(int(uint32_t(total)), m, kWave));
+        total = waveGroupReduce<kWave, SumOp>(total) * 1.02f;
         fine = !__any(!fine);
         if (report && !fine && lane == 0) atomicOr(a.err, kErrPagedIndex);
         // row starts that go back may make more items than the grid has: a tile whose chunks did not all run
         // would leave its counter behind, so nothing is split then
         if (a.target && fine) {
-            const uint64_t want = (total * unsigned(a.heads) + a.target - 1) / a.target, up = (want + kLeast - 1) / kLeast * kLeast;
-            per = up < kLeast ? kLeast : (up < kAll ? unsigned(up) : kAll);
+            const float want = total * float(a.heads) * a.per_target;
+            per = want < 0x1p30f ? (unsigned(want) / kLeast + 1) * kLeast : kAll;
         }
     }
-    unsigned items = 0, splits = 0; // before this group of requests
+    per = unsigned(uniform(int(per)));
+    int items = 0, splits = 0; // before this group of requests
     for (int64_t r0 = 0; r0 < a.requests; r0 += kWave) {
-        request(r0 + lane, start, n, len);
-        const unsigned tiles = tilesOf(n), steps = stepsOf(len), chunks = steps > per ? (steps + per - 1) / per : 1;
+        if (r0) request(r0 + lane, q);
+        else q = first;
+        const unsigned tiles = tilesOf(q), steps = stepsOf(q);
+        unsigned chunks = 1;
+        if (__any(steps > per)) chunks = steps > per ? (steps + per - 1) / per : 1;
         const unsigned mine = tiles * chunks, split = chunks > 1 ? mine : 0;
-        unsigned to = mine, sto = split;
-#pragma unroll
-        for (int d = 1; d < kWave; d <<= 1) {
-            const unsigned u = __shfl_up(to, d, kWave), v = __shfl_up(sto, d, kWave);
-            to += lane >= d ? u : 0;
-            sto += lane >= d ? v : 0;
-        }
-        const uint64_t hit = __ballot(index >= items + to - mine && index < items + to);
+        const unsigned to = waveScan(mine), sto = __any(chunks > 1) ? waveScan(split) : 0;
+        const unsigned at = unsigned(index - items); // before the group where it wraps
+        const uint64_t hit = __ballot(at >= to - mine && at < to);
         if (hit) {
             const int l = uniform(__ffsll(static_cast<unsigned long long>(hit)) - 1);
-            const auto of = [&](unsigned v) { return unsigned(__builtin_amdgcn_readlane(int(v), l)); };
-            const unsigned in = unsigned(uniform(int(index - items))) - of(to - mine), c = of(chunks), t = in / c;
+            const auto of = [&](unsigned v) { return __builtin_amdgcn_readlane(int(v), l); };
             // one value for the wave in every field: scalar registers, and branches that are no masks
+            const int in = uniform(index - items) - of(to - mine), c = of(chunks), t = c == 1 ? in : in / c;
             Item it;
             it.any = true;
             it.request = uniform(int(r0)) + l;
-            it.start = int(of(unsigned(start)));
-            it.n = int(of(unsigned(n)));
-            it.len = int(of(unsigned(len)));
-            it.tile = int(of(tiles) - 1 - t); // the last sees most keys: first
-            it.chunk = int(in - t * c);
-            it.chunks = int(c);
-            it.step0 = it.chunk * uniform(int(per));
-            it.step1 = c == 1 ? int(kAll) : it.step0 + uniform(int(per));
-            it.split = unsigned(uniform(int(splits))) + of(sto - split) + t * c;
+            it.start = of(unsigned(q.start));
+            it.n = of(unsigned(q.n));
+            it.len = of(unsigned(q.len));
+            it.tile = of(tiles) - 1 - t; // the last sees most keys: first
+            it.chunk = in - t * c;
+            it.chunks = c;
+            it.step0 = it.chunk * int(per);
+            it.step1 = c == 1 ? int(kAll) : it.step0 + int(per);
+            it.split = unsigned(uniform(splits) + of(sto - split) + t * c);
             return it;
         }
-        const auto last = [](unsigned v) { return unsigned(__builtin_amdgcn_readlane(int(v), kWave - 1)); };
-        items += last(to);
-        splits += last(sto);
+        items += __builtin_amdgcn_readlane(int(to), kWave - 1);
+        splits += __builtin_amdgcn_readlane(int(sto), kWave - 1);
     }
     Item none{};
     return none;

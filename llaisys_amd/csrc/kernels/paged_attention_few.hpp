@@ -19,19 +19,18 @@ struct QueryRows {
     static constexpr bool kTwo = std::is_same_v<T, F32>;
     v8h hi[NT][2], lo[kTwo ? NT : 1][2];
     int exponent;
-    __device__ void load(const PagedAttnArgs &a, bool valid, size_t elem, int quarter) {
-        float f[NT][2][8];
+    __device__ __forceinline__ void set(const Raw8<T> (&raw)[NT][2]) {
+        exponent = 0;
+        if constexpr (std::is_same_v<T, F16>) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) hi[t][h] = __builtin_bit_cast(v8h, raw[t][h].r[0]);
+            return;
+        }
         float top = 0.0f;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int c = 64 * t + 16 * quarter + 8 * h;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) f[t][h][e] = 0.0f;
-                if (valid && c < a.dim) load8<T>(a.q, elem + c, f[t][h]);
-                top = foldFinite(top, f[t][h]);
-            }
+        for (int t = 0; t < NT; ++t) top = fmaxf(top, largest(raw[t]));
         top = butterflyStep<16, MaxOp>(top);
         top = butterflyStep<32, MaxOp>(top);
         exponent = rowExponent(top);
@@ -39,10 +38,12 @@ struct QueryRows {
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
+                float f[8];
+                raw[t][h].unpack(f);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[t][h][e] = __builtin_amdgcn_ldexpf(f[t][h][e], exponent);
-                if constexpr (kTwo) split8(f[t][h], hi[t][h], lo[t][h]);
-                else hi[t][h] = narrow8(f[t][h]);
+                for (int e = 0; e < 8; ++e) f[e] = __builtin_amdgcn_ldexpf(f[e], exponent);
+                if constexpr (kTwo) split8(f, hi[t][h], lo[t][h]);
+                else hi[t][h] = narrow8(f);
             }
     }
 };
@@ -70,23 +71,20 @@ __global__ __launch_bounds__(kPagedThreads, NT <= 2 ? 2 : 1) void pagedFew(Paged
     __shared__ unsigned arrived;
     const int dim = D ? D : a.dim;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave), lane = int(threadIdx.x) % kWave;
-    const int m16 = lane % 16, quarter = lane / 16, head = int(blockIdx.x % unsigned(a.heads));
-    Item it = findItem<kRows>(a, blockIdx.x / unsigned(a.heads), blockIdx.x == 0 && wave == 0);
+    const int m16 = lane % 16, quarter = lane / 16, index = a.by_heads.div(int(blockIdx.x)), head = int(blockIdx.x) - index * a.heads;
+    Item it = findItem<kRows>(a, index, blockIdx.x == 0 && wave == 0);
     if (!it.any) return;
 
     const int first_row = it.tile * kRows, rows = min(kRows, it.n * a.group - first_row);
-    const int row = first_row + m16, token = row / a.group;
+    const int row = first_row + m16, token = a.by_group.div(row);
     const int before = it.len - it.n; // tokens cached before the rows; a row sees before + token + 1
-    const int seen_last = before + (first_row + rows - 1) / a.group + 1, seen_first = before + first_row / a.group + 1;
+    const int seen_last = before + a.by_group.div(first_row + rows - 1) + 1, seen_first = before + a.by_group.div(first_row) + 1;
     const int steps = seen_last > 0 ? (seen_last + kStep - 1) / kStep : 0;
     if (!cutItem(it, steps)) return;
     const int end = min(it.step1, steps);
     const int limit = before + token + 1;
-    const int token0 = first_row / a.group, out_row = (token - token0) * a.nh + head * a.group + (row - token * a.group);
+    const int token0 = a.by_group.div(first_row), out_row = (token - token0) * a.nh + head * a.group + (row - token * a.group);
     const size_t out0 = size_t(it.start + token0) * a.nh;
-    QueryRows<T, NT> q;
-    q.load(a, m16 < rows, (out0 + unsigned(out_row)) * dim, quarter);
-    const float row_scale = __builtin_amdgcn_ldexpf(a.scale * kLog2e, 9 - q.exponent);
 
     const int32_t *table = a.table + int64_t(it.request) * a.width;
     const int in_block = (1 << a.shift) - 1;
@@ -123,6 +121,8 @@ __global__ __launch_bounds__(kPagedThreads, NT <= 2 ? 2 : 1) void pagedFew(Paged
         if (d.bad && step * kStep + 16 * quarter < seen_last) atomicOr(a.err, kErrPagedIndex);
     };
 
+    QueryRows<T, NT> q;
+    float row_scale = 0.0f;
     float mx = -INFINITY, l = 0.0f, vref = 0.0f;
     v4f acc[CH];
 #pragma unroll
@@ -205,7 +205,24 @@ __global__ __launch_bounds__(kPagedThreads, NT <= 2 ? 2 : 1) void pagedFew(Paged
         }
     };
 
+    // the rows, loaded while the first keys' ids are on their way, and made operands while their codes are
     int step = it.step0 + wave;
+    Ids now{0, 0};
+    if (step < end) now = ids(step);
+    Raw8<T> raw[NT][2];
+    const size_t row_at = (out0 + unsigned(out_row)) * dim;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int c = 64 * t + 16 * quarter + 8 * h;
+            if (m16 < rows && c < dim) raw[t][h].load(a.q, row_at + c);
+            else raw[t][h].zero();
+        }
+    const auto setRows = [&] {
+        q.set(raw);
+        row_scale = __builtin_amdgcn_ldexpf(a.scale * kLog2e, 9 - q.exponent);
+    };
     if constexpr (kAhead) {
         StepData<NT> d0, d1;
         Ids next{0, 0};
@@ -215,9 +232,10 @@ __global__ __launch_bounds__(kPagedThreads, NT <= 2 ? 2 : 1) void pagedFew(Paged
             if (step + 2 * NW < end) next = ids(step + 2 * NW);
         };
         if (step < end) {
-            fetch(step, ids(step), d0);
+            fetch(step, now, d0);
             if (step + NW < end) next = ids(step + NW);
         }
+        setRows();
         for (; step < end; step += NW) {
             fetchNext(d1);
             compute(step, d0);
@@ -227,9 +245,11 @@ __global__ __launch_bounds__(kPagedThreads, NT <= 2 ? 2 : 1) void pagedFew(Paged
             compute(step, d1);
         }
     } else {
+        setRows();
         for (; step < end; step += NW) {
             StepData<NT> d;
-            fetch(step, ids(step), d);
+            fetch(step, now, d);
+            if (step + NW < end) now = ids(step + NW);
             compute(step, d);
         }
     }

@@ -59,52 +59,26 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
     __shared__ unsigned arrived;
     const int dim = D ? D : a.dim;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave), lane = int(threadIdx.x) % kWave;
-    const int col = lane % 32, half = lane / 32, head = int(blockIdx.x % unsigned(a.heads));
-    Item it = findItem<kManyTile>(a, blockIdx.x / unsigned(a.heads), blockIdx.x == 0 && wave == 0);
+    const int col = lane % 32, half = lane / 32, index = a.by_heads.div(int(blockIdx.x)), head = int(blockIdx.x) - index * a.heads;
+    Item it = findItem<kManyTile>(a, index, blockIdx.x == 0 && wave == 0);
     if (!it.any) return;
 
     const int total_rows = it.n * a.group;
     const int first_row = it.tile * kManyTile, rows = min(kManyTile, total_rows - first_row);
     const int before = it.len - it.n;
-    const auto seenBy = [&](int row) { return before + row / a.group + 1; };
+    const auto seenBy = [&](int row) { return before + a.by_group.div(row) + 1; };
     const int seen_last = seenBy(first_row + rows - 1);
     const int steps = seen_last > 0 ? (seen_last + kStep - 1) / kStep : 0;
     if (!cutItem(it, steps)) return;
     const int end = min(it.step1, steps);
 
     // this wave's rows
-    const int wrow = first_row + 32 * wave, row = wrow + col, token = row / a.group;
+    const int wrow = first_row + 32 * wave, row = wrow + col, token = a.by_group.div(row);
     const bool valid = row < total_rows;
     const int limit = before + token + 1;
     const int wave_last = wrow < total_rows ? seenBy(min(wrow + 31, total_rows - 1)) : 0, wave_first = seenBy(wrow);
-    const int token0 = first_row / a.group, out_row = (token - token0) * a.nh + head * a.group + (row - token * a.group);
+    const int token0 = a.by_group.div(first_row), out_row = (token - token0) * a.nh + head * a.group + (row - token * a.group);
     const size_t out0 = size_t(it.start + token0) * a.nh;
-    v8h q[kSteps], ql[kTwoQ ? kSteps : 1];
-    float row_scale;
-    {
-        const size_t at = (out0 + unsigned(out_row)) * dim + 8 * half;
-        const float sign = a.scale < 0.0f ? -1.0f : 1.0f; // the scale of a score is not negative below
-        float top = 0.0f;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            float f[8] = {};
-            if (valid && 16 * s < dim) load8<T>(a.q, at + 16 * s, f);
-            top = foldFinite(top, f);
-        }
-        top = butterflyStep<32, MaxOp>(top);
-        const int e = rowExponent(top);
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            float f[8] = {};
-            if (valid && 16 * s < dim) load8<T>(a.q, at + 16 * s, f); // again, from the cache: 8 values at a time in registers
-#pragma unroll
-            for (int x = 0; x < 8; ++x) f[x] = __builtin_amdgcn_ldexpf(sign * f[x], e);
-            if constexpr (kTwoQ) split8(f, q[s], ql[s]);
-            else q[s] = narrow8(f);
-        }
-        row_scale = __builtin_amdgcn_ldexpf(fabsf(a.scale) * kLog2e, 9 - e);
-    }
-
     // ---- the wave's 16 keys of a tile: HBM -> registers -> LDS
     const int32_t *table = a.table + int64_t(it.request) * a.width;
     const size_t tile_bytes = size_t(dim) << a.shift;
@@ -143,6 +117,40 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
         vs = a.v_scale[tile];
         id_next = idOf(step + 1);
     };
+    // The rows, loaded while the first keys' ids are on their way, and made operands while their codes are.
+    if (it.step0 < end) id_next = idOf(it.step0);
+    v8h q[kSteps], ql[kTwoQ ? kSteps : 1];
+    float row_scale;
+    {
+        Raw8<T> raw[kSteps];
+        const size_t at = (out0 + unsigned(out_row)) * dim + 8 * half;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            if (valid && (D || 16 * s < dim)) raw[s].load(a.q, at + 16 * s);
+            else raw[s].zero();
+        }
+        if (it.step0 < end) fetch(it.step0);
+        // the scale of a score is not negative below: its sign goes to the rows
+        int e = 0;
+        if constexpr (std::is_same_v<T, F16>) {
+            const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) q[s] = __builtin_bit_cast(v8h, raw[s].r[0] ^ flip);
+        } else {
+            const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
+            e = rowExponent(butterflyStep<32, MaxOp>(largest(raw)));
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                float f[8];
+                raw[s].unpack(f);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) f[x] = __builtin_amdgcn_ldexpf(sign * f[x], e);
+                if constexpr (kTwoQ) split8(f, q[s], ql[s]);
+                else q[s] = narrow8(f);
+            }
+        }
+        row_scale = __builtin_amdgcn_ldexpf(fabsf(a.scale) * kLog2e, 9 - e);
+    }
     const auto put16 = [&](int at, const v8h &x) { *reinterpret_cast<v8h *>(sh.in + at) = x; };
     const auto get16 = [&](int at) { return *reinterpret_cast<const v8h *>(sh.in + at); };
     // places in the buffers, of the next step to write and the next to read
@@ -328,8 +336,6 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
     };
 
     if (it.step0 < end) {
-        id_next = idOf(it.step0);
-        fetch(it.step0);
         stage();
         fetch(it.step0 + 1);
         ldsBarrier();
