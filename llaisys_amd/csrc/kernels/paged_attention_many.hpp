@@ -92,17 +92,30 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
     int id_next = 0;
     // past the item's keys these read keys of its last block again
     const auto idOf = [&](int step) { return table[min(step * kStep + 16 * wave, seen_last - 1) >> a.shift]; };
-    const auto fetch = [&](int step) { // uses id_next, and reads the id after it
+    struct Place {
+        const int8_t *k, *v;
+        const float *ks, *vs;
+        bool bad;
+    };
+    const auto placeOf = [&](int step) { // of the step whose id is id_next
         const int id = uniform(id_next);
-        bad = uint32_t(id) >= uint32_t(a.n_blocks);
-        any_bad = any_bad || (bad && step * kStep + 16 * wave < seen_last);
-        const int64_t tile = (bad ? 0 : int64_t(id)) * a.heads + head;
+        Place p;
+        p.bad = uint32_t(id) >= uint32_t(a.n_blocks);
+        any_bad = any_bad || (p.bad && step * kStep + 16 * wave < seen_last);
+        const int64_t tile = (p.bad ? 0 : int64_t(id)) * a.heads + head;
         const size_t at = tile * tile_bytes + size_t((step * kStep + 16 * wave) & in_block) * dim;
-        const int8_t *kp = a.k_codes + at, *vp = a.v_codes + at;
+        p.k = a.k_codes + at;
+        p.v = a.v_codes + at;
+        p.ks = a.k_scale + tile;
+        p.vs = a.v_scale + tile;
+        return p;
+    };
+    const auto fetch = [&](int step, const Place &p) {
+        id_next = idOf(step + 1); // first, as it is needed first
         int c = 16 * k_piece;
         if (D != DP) c = c < dim ? c : 0; // behind the row: q is 0 there
 #pragma unroll
-        for (int i = 0; i < kK; ++i) kr[i] = *reinterpret_cast<const v4u *>(kp + unsigned((k_key + i * (1024 / DP)) * dim + c));
+        for (int i = 0; i < kK; ++i) kr[i] = *reinterpret_cast<const v4u *>(p.k + unsigned((k_key + i * (1024 / DP)) * dim + c));
         if (DP >= 128 || lane < 32) {
 #pragma unroll
             for (int u = 0; u < kV; ++u) {
@@ -110,12 +123,12 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
                 if (D != DP) ch = ch < dim ? ch : 0; // not stored
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    vr[u][i] = *reinterpret_cast<const uint32_t *>(vp + unsigned((8 * (v_chunk + u) + i) * dim + ch));
+                    vr[u][i] = *reinterpret_cast<const uint32_t *>(p.v + unsigned((8 * (v_chunk + u) + i) * dim + ch));
             }
         }
-        ks = a.k_scale[tile];
-        vs = a.v_scale[tile];
-        id_next = idOf(step + 1);
+        ks = *p.ks;
+        vs = *p.vs;
+        bad = p.bad;
     };
     // The rows, loaded while the first keys' ids are on their way, and made operands while their codes are.
     if (it.step0 < end) id_next = idOf(it.step0);
@@ -129,7 +142,7 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
             if (valid && (D || 16 * s < dim)) raw[s].load(a.q, at + 16 * s);
             else raw[s].zero();
         }
-        if (it.step0 < end) fetch(it.step0);
+        if (it.step0 < end) fetch(it.step0, placeOf(it.step0));
         // the scale of a score is not negative below: its sign goes to the rows
         int e = 0;
         if constexpr (std::is_same_v<T, F16>) {
@@ -158,28 +171,32 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
     int v_to = Sh::kV + 4 * v_quad * kStep * 2 + vColumn(4 * v_quad, 2 * wave + v_chunk) * 16;
     int s_to = Sh::kScales + (lane == 0 ? wave * 16 : 128 + lane * 16);
     const int s_flip = lane == 0 ? 64 : 0;
-    // The staging in pieces, to be put between products: 2 kK of K, 4 kV of V.
-    constexpr int kPieces = 2 * kK + 4 * kV;
+    // The staging in halves of 16-byte pieces, to be put between products: 2 kK pieces of K, 4 kV of V.
+    constexpr int kHalves = 2 * (2 * kK + 4 * kV);
     uint32_t vx[kV][8];
-    const auto stagePiece = [&](int j) {
+    Pairs piece;
+    const auto stageHalf = [&](int n) {
+        const int j = n / 2, h = n % 2;
         if (j < 2 * kK) {
             // keys 1024 / DP apart: bit 2 of the key, where it changes, moves the column
             const int i = j / 2, at = k_to ^ (DP == 256 ? (i & 1) * 128 : 0) ^ (j % 2 * 16);
-            put16(at + i * 2048, j % 2 ? codes8(kr[i].z, kr[i].w) : codes8(kr[i].x, kr[i].y));
+            const uint32_t w = (j % 2 ? (h ? kr[i].w : kr[i].z) : (h ? kr[i].y : kr[i].x)) ^ 0x80808080u;
+            piece.p[2 * h] = codePair(__builtin_amdgcn_perm(w, w, 0x0c010c00u));
+            piece.p[2 * h + 1] = codePair(__builtin_amdgcn_perm(w, w, 0x0c030c02u));
+            if (h) put16(at + i * 2048, join(piece));
             return;
         }
         const int u = (j - 2 * kK) / 4, x = (j - 2 * kK) % 4;
         constexpr uint32_t kSel[4] = {0x0c040c00u, 0x0c050c01u, 0x0c060c02u, 0x0c070c03u};
         if (x == 0) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) vx[u][i] = vr[u][i] ^ 0x80808080u;
+            for (int i = 4 * h; i < 4 * h + 4; ++i) vx[u][i] = vr[u][i] ^ 0x80808080u;
         }
-        Pairs p;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) p.p[e] = codePair(__builtin_amdgcn_perm(vx[u][2 * e + 1], vx[u][2 * e], kSel[x]));
+        for (int e = 2 * h; e < 2 * h + 2; ++e) piece.p[e] = codePair(__builtin_amdgcn_perm(vx[u][2 * e + 1], vx[u][2 * e], kSel[x]));
         // (of 64 channels half the lanes have none: theirs go behind the scales)
         const int at = (v_to ^ (u * 16) ^ (x / 2 * 64)) + x * kStep * 2;
-        put16(DP >= 128 || lane < 32 ? at : Sh::kScales + 128 + lane * 16, join(p));
+        if (h) put16(DP >= 128 || lane < 32 ? at : Sh::kScales + 128 + lane * 16, join(piece));
     };
     const auto stageScales = [&] {
         const float v = checkedScale(vs);
@@ -191,7 +208,7 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
     };
     const auto stage = [&] {
 #pragma unroll
-        for (int j = 0; j < kPieces; ++j) stagePiece(j);
+        for (int j = 0; j < kHalves; ++j) stageHalf(j);
         stageScales();
     };
 
@@ -207,35 +224,45 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
     int v_from = Sh::kV + col * kStep * 2 + vColumn(col, 2 * half) * 16;
     int s_from = Sh::kScales;
 
-    // The next step's codes are staged beside the first product, those of the one after it asked for.  `hide`: some row of
-    // the wave does not see some key of the step.
-    const auto compute = [&](int step, const v4u (&info)[4], bool hide) {
+    // The next step's codes are staged beside the first product, and those of the one after it asked for.
+    const auto compute = [&](int step) {
+        const Place place = placeOf(step + 2);
+        v4u info[4];
         v16f sc[2];
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[0][i] = sc[1][i] = 0.0f;
-        // operands two products ahead, a piece of the staging before each product
-        v8h k[3][2];
-        const auto readK = [&](int x) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) k[x % 3][t] = get16((k_from ^ (x * 32)) + t * 32 * DP * 2);
+        float best[2] = {-INFINITY, -INFINITY};
+        // operands three products ahead, half a piece of the staging before each; the first 32 keys' maximum beside the
+        // product of the others
+        constexpr int kRingK = 4;
+        v8h k[kRingK];
+        const auto readK = [&](int n) {
+            if (n < 2 * kSteps) k[n % kRingK] = get16((k_from ^ (n % kSteps * 32)) + n / kSteps * 32 * DP * 2);
         };
-        readK(0);
-        if constexpr (kSteps > 1) readK(1);
 #pragma unroll
-        for (int x = 0; x < kSteps; ++x) {
-            if (x + 2 < kSteps) readK(x + 2);
+        for (int n = 0; n < kRingK - 1; ++n) readK(n);
 #pragma unroll
-            for (int j = x * kPieces / kSteps; j < (x + 1) * kPieces / kSteps; ++j) stagePiece(j);
-            __builtin_amdgcn_sched_barrier(0);
+        for (int g = 0; g < 4; ++g) info[g] = *reinterpret_cast<const v4u *>(sh.in + s_from + 16 * g);
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[x % 3][t], q[x], sc[t], 0, 0, 0);
-                if constexpr (kTwoQ) sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[x % 3][t], ql[x], sc[t], 0, 0, 0);
+        for (int n = 0; n < 2 * kSteps; ++n) {
+            const int t = n / kSteps, x = n % kSteps;
+            readK(n + kRingK - 1);
+#pragma unroll
+            for (int j = n * kHalves / (2 * kSteps); j < (n + 1) * kHalves / (2 * kSteps); ++j) stageHalf(j);
+            if (t == 1) {
+#pragma unroll
+                for (int i = x * 16 / kSteps; i < (x + 1) * 16 / kSteps; ++i) best[0] = fmaxf(best[0], sc[0][i]);
             }
+            __builtin_amdgcn_sched_barrier(0);
+            sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[n % kRingK], q[x], sc[t], 0, 0, 0);
+            if constexpr (kTwoQ) sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[n % kRingK], ql[x], sc[t], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
         stageScales();
-        fetch(step + 2);
+        fetch(step + 2, place);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) best[1] = fmaxf(best[1], sc[1][i]);
+        const bool hide = (step + 1) * kStep > wave_first || uniform(int(info[0].w | info[1].w | info[2].w | info[3].w)) != 0;
         // this lane's keys: 32 t + 16 half + 0..15
         float c[2], vscale[2], shift[2];
         bool sees[2] = {true, true};
@@ -256,16 +283,16 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     if (i >= left) sc[t][i] = -3e38f;
+                best[t] = sc[t][0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) best[t] = fmaxf(best[t], sc[t][i]);
                 if (c[t] < 1e-30f || !sees[t]) c[t] = 1e-30f;
             }
         }
         float top = -INFINITY, vtop = vref;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            float best = sc[t][0];
-#pragma unroll
-            for (int i = 1; i < 16; ++i) best = fmaxf(best, sc[t][i]);
-            top = sees[t] ? fmaxf(top, best * c[t]) : top;
+            top = sees[t] ? fmaxf(top, best[t] * c[t]) : top;
             vtop = sees[t] ? fmaxf(vtop, vscale[t]) : vtop;
         }
         top = butterflyStep<32, MaxOp>(top);
@@ -337,18 +364,14 @@ __global__ __launch_bounds__(kPagedThreads, (kManyBlocks<T, DP>)) void pagedMany
 
     if (it.step0 < end) {
         stage();
-        fetch(it.step0 + 1);
+        fetch(it.step0 + 1, placeOf(it.step0 + 1));
         ldsBarrier();
         for (int step = it.step0; step < end; ++step) {
             if (step * kStep < wave_last) {
-                v4u info[4];
-#pragma unroll
-                for (int g = 0; g < 4; ++g) info[g] = *reinterpret_cast<const v4u *>(sh.in + s_from + 16 * g);
-                const bool none = uniform(int(info[0].w | info[1].w | info[2].w | info[3].w)) != 0;
-                compute(step, info, none || (step + 1) * kStep > wave_first);
+                compute(step);
             } else {
                 stage();
-                fetch(step + 2);
+                fetch(step + 2, placeOf(step + 2));
             }
             k_from ^= Sh::kBuffer;
             v_from ^= Sh::kBuffer;
