@@ -8,10 +8,14 @@
 // while it fills; each growth rounds its older codes once more, by at most s / 2.
 //
 // Quotients are rounded as the exact quotient rounds (ties to even), so that one definition holds for any
-// way of computing it: with n = rint(x * (1 / s)), off by at most one, e = fma(-n, s, x) is exact, and n
-// moves by one where |e| > s / 2, or |e| = s / 2 with n odd.  (|n| < 2^8: n * s and x * 2^k / s agree in all but
-// the last bits, so e needs no more than 24 bits.)  Scales below 2^-96, where 1 / s or e may leave the
-// normal range, divide in f64, and so do the older codes.
+// way of computing it: with n the whole number next to x * (1 / s), off by at most one, e = fma(-n, s, x) is
+// exact (x and n * s agree in all but the last bits), and n is right wherever |e| < s / 2.  Elsewhere (ties, quotients next
+// to one, NaN), and for scales below 2^-96, where 1 / s or e may leave the normal range, the quotient is taken in f64, which
+// tells any two of them from a half apart; so are the older codes.
+//
+// A group of 256 threads takes `chunk` rows of one head of k or v.  Its slots come in one load of 64, in which every
+// wave finds the rows where cache blocks begin and how far they go; rows stay in registers between the maximum and
+// the codes.  [7598 x 8 heads x 128] bf16, k and v (47 MB): CHUNK_US us.
 #include "common.hpp"
 #include "launch.hpp"
 #include "quantize.hpp"
@@ -30,17 +34,9 @@ struct AppendArgs {
     const int64_t *slots;
     int64_t rows, slot_end;
     int heads, dim, shift, chunk;
+    DivU64 by_vectors; // of a row
     int *err;
 };
-
-__device__ __forceinline__ float codeFast(float x, float s, float recip) {
-    float n = rintf(x * recip);
-    const float e = __builtin_fmaf(-n, s, x), h = 0.5f * s;
-    const bool odd = (int(n) & 1) != 0;
-    if (e > h || (e == h && odd)) n += 1.0f;
-    if (e < -h || (e == -h && odd)) n -= 1.0f;
-    return n;
-}
 
 __device__ __forceinline__ uint32_t codeExact(double x, double s) {
     double n = rint(x / s);
@@ -49,21 +45,25 @@ __device__ __forceinline__ uint32_t codeExact(double x, double s) {
     return uint32_t(int32_t(n)) & 0xFFu;
 }
 
-// Codes of one 16-byte vector; s is the block's scale, fast where the f32 rule holds.
+// Codes of one 16-byte vector; s is the block's scale, recip 1 / s, or NaN where the f32 rule does not hold.
 template <typename T>
-__device__ __forceinline__ void storeVec(int8_t *to, const v4u &r, float s, float recip, bool fast) {
+__device__ __forceinline__ void storeVec(int8_t *to, const v4u &r, float s, float recip) {
     constexpr int N = Fmt<T>::kVec;
+    constexpr float kWhole = 12582912.0f; // 1.5 * 2^23: a sum with it rounds to a whole number, in its low bits
     float f[N];
     Fmt<T>::unpack(r, f);
     uint32_t c[N];
+    const float half = 0.5f * s;
+    bool near = true;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-        if (fast) {
-            const float n = codeFast(f[e], s, recip);
-            c[e] = n == n ? uint32_t(int32_t(n)) & 0xFFu : 0u;
-        } else {
-            c[e] = codeExact(f[e], s);
-        }
+        const float m = __builtin_fmaf(f[e], recip, kWhole), rest = __builtin_fmaf(kWhole - m, s, f[e]);
+        near = near && fabsf(rest) < half;
+        c[e] = __float_as_uint(m);
+    }
+    if (__builtin_expect(!near, 0)) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) c[e] = codeExact(f[e], s);
     }
     uint32_t w[N / 4];
 #pragma unroll
@@ -71,73 +71,85 @@ __device__ __forceinline__ void storeVec(int8_t *to, const v4u &r, float s, floa
     __builtin_memcpy(__builtin_assume_aligned(to, N), w, N);
 }
 
-// A block of threads takes `chunk` rows of one head of k or v, and of them the rows where a cache block begins.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void pagedAppend(AppendArgs a) {
     constexpr int N = Fmt<T>::kVec;
     constexpr int kKeep = 8; // vectors a thread keeps between the maximum and the codes
     __shared__ float red[kThreads / kWave];
-    __shared__ int run_end;
-    const int head = blockIdx.y, kv = blockIdx.z;
+    const int head = blockIdx.y, kv = blockIdx.z, lane = threadIdx.x % kWave;
     const int nv = a.dim / N, block = 1 << a.shift;
-    const int64_t t_end = min(a.rows, (int64_t(blockIdx.x) + 1) * a.chunk);
-    for (int64_t t = int64_t(blockIdx.x) * a.chunk; t < t_end; ++t) {
-        const int64_t slot = a.slots[t];
-        if (slot < 0) continue;
-        if (slot >= a.slot_end) {
-            if (threadIdx.x == 0) atomicOr(a.err, kErrPagedIndex);
-            continue;
-        }
-        const int64_t id = slot >> a.shift;
-        if (t > 0 && a.slots[t - 1] >= 0 && (a.slots[t - 1] >> a.shift) == id) continue; // not the block's first row
+    // slots t0 - 1 .. t0 + 62; the rows of lanes 1 .. chunk are this group's
+    const int64_t t0 = int64_t(blockIdx.x) * a.chunk;
+    const auto slotAt = [&](int64_t t) { return t >= 0 && t < a.rows ? a.slots[t] : int64_t(-1); };
+    const int64_t mine = slotAt(t0 - 1 + lane);
+    const bool ours = lane >= 1 && lane <= a.chunk;
+    if (ours && mine >= a.slot_end) atomicOr(a.err, kErrPagedIndex);
+    const int64_t my_block = mine < 0 ? -1 : mine >> a.shift;
+    const auto pick = [](int64_t v, int l) {
+        return int64_t((uint64_t(uint32_t(__builtin_amdgcn_readlane(int(v >> 32), l))) << 32) | uint32_t(__builtin_amdgcn_readlane(int(v), l)));
+    };
+    const int64_t before = (int64_t(__shfl_up(int(my_block >> 32), 1, kWave)) << 32) | uint32_t(__shfl_up(int(my_block), 1, kWave));
+    for (uint64_t firsts = __ballot(ours && mine >= 0 && mine < a.slot_end && my_block != before); firsts; firsts &= firsts - 1) {
+        const int l = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(firsts)) - 1);
+        const int64_t t = t0 - 1 + l, slot = pick(mine, l), id = slot >> a.shift;
+        const int first = int(slot & (block - 1));
         // the run of rows of this block; rows that do not follow each other are refused
-        __syncthreads();
-        if (threadIdx.x == 0) run_end = block + 1;
-        __syncthreads();
-        bool follows = true;
-        for (int i = threadIdx.x; i <= block; i += kThreads) {
-            const int64_t st = t + i < a.rows ? a.slots[t + i] : -1;
-            if (st < 0 || (st >> a.shift) != id)
-                atomicMin(&run_end, i);
+        int run = 0;
+        bool refuse = false;
+        int64_t window = mine;
+        for (int at = l;; at -= kWave) { // `at`: lane of row t in the window
+            const int i = lane - at;     // rows behind t
+            const bool ends = i >= 1 && (first + i >= block || window != slot + i);
+            const uint64_t m = __ballot(ends);
+            if (m) {
+                const int stop = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(m)) - 1);
+                const int64_t other = pick(window, stop);
+                run = stop - at;
+                refuse = other >= 0 && (other >> a.shift) == id;
+                break;
+            }
+            window = slotAt(t + (kWave - at) + lane);
         }
-        __syncthreads();
-        const int run = run_end;
-        for (int i = threadIdx.x; i < run; i += kThreads) follows = follows && a.slots[t + i] == slot + i;
-        if (!__syncthreads_and(follows)) {
+        if (refuse) {
             if (threadIdx.x == 0) atomicOr(a.err, kErrPagedIndex);
             continue;
         }
-        const int first = int(slot & (block - 1)), n = run * nv;
+        const int n = run * nv;
         const char *in = static_cast<const char *>(a.in[kv]);
         const auto at = [&](int j) {
-            const int row = j / nv;
+            const int row = int(a.by_vectors.div(uint64_t(j)));
             return (size_t(t + row) * a.heads + head) * a.dim + size_t(j - row * nv) * N;
         };
+        const size_t tile = size_t(id) * a.heads + head;
+        const float s0 = first ? a.scale[kv][tile] : 0.0f;
         v4u keep[kKeep];
-        float amax = 0.0f;
-        const auto fold = [&](const v4u &r) {
-            float f[N];
-            Fmt<T>::unpack(r, f);
-#pragma unroll
-            for (int e = 0; e < N; ++e) amax = MaxOp::apply(amax, fabsf(f[e]));
-        };
 #pragma unroll
         for (int i = 0; i < kKeep; ++i) {
             const int j = threadIdx.x + i * kThreads;
-            keep[i] = j < n ? load16<T>(in, at(j)) : v4u{0, 0, 0, 0};
+            keep[i] = j < n ? load16Stream<T>(in, at(j)) : v4u{0, 0, 0, 0};
         }
+        uint32_t bits = 0;
 #pragma unroll
-        for (int i = 0; i < kKeep; ++i) fold(keep[i]);
-        for (int j = threadIdx.x + kKeep * kThreads; j < n; j += kThreads) fold(load16<T>(in, at(j)));
-        const size_t tile = size_t(id) * a.heads + head;
-        const float s0 = first ? a.scale[kv][tile] : 0.0f;
+        for (int i = 0; i < kKeep; ++i) bits = AbsBits<T>::fold(bits, keep[i]);
+        for (int j = threadIdx.x + kKeep * kThreads; j < n; j += kThreads) bits = AbsBits<T>::fold(bits, load16<T>(in, at(j)));
+        bits = AbsBits<T>::finish(bits);
+        float amax = AbsBits<T>::value(bits);
+        if (__builtin_expect(bits > AbsBits<T>::kInf, 0)) { // a NaN, which never raises the maximum
+            amax = 0.0f;
+            for (int j = threadIdx.x; j < n; j += kThreads) {
+                float f[N];
+                Fmt<T>::unpack(load16<T>(in, at(j)), f);
+#pragma unroll
+                for (int e = 0; e < N; ++e) amax = MaxOp::apply(amax, fabsf(f[e]));
+            }
+        }
         amax = groupReduce<kThreads, MaxOp>(amax, red);
         const float grown = amax / 127.0f, s = grown > s0 ? grown : s0;
         int8_t *codes = a.codes[kv] + (tile << a.shift) * a.dim;
         if (threadIdx.x == 0 && (s != s0 || first == 0)) a.scale[kv][tile] = s;
         if (first && s != s0) {
             for (int j = threadIdx.x; j < first * (a.dim / 16); j += kThreads) {
-                v4u r = *reinterpret_cast<const v4u *>(codes + j * 16);
+                const v4u r = *reinterpret_cast<const v4u *>(codes + j * 16);
                 uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -150,15 +162,14 @@ __global__ __launch_bounds__(kThreads) void pagedAppend(AppendArgs a) {
                 *reinterpret_cast<v4u *>(codes + j * 16) = v4u{w[0], w[1], w[2], w[3]};
             }
         }
-        const float recip = 1.0f / s;
-        const bool fast = s >= 0x1p-96f && s <= 0x1p120f;
+        const float recip = s >= 0x1p-96f && s <= 0x1p120f ? 1.0f / s : __builtin_nanf("");
 #pragma unroll
         for (int i = 0; i < kKeep; ++i) {
             const int j = threadIdx.x + i * kThreads;
-            if (j < n) storeVec<T>(codes + first * a.dim + j * N, keep[i], s, recip, fast);
+            if (j < n) storeVec<T>(codes + first * a.dim + j * N, keep[i], s, recip);
         }
         for (int j = threadIdx.x + kKeep * kThreads; j < n; j += kThreads)
-            storeVec<T>(codes + first * a.dim + j * N, load16<T>(in, at(j)), s, recip, fast);
+            storeVec<T>(codes + first * a.dim + j * N, load16<T>(in, at(j)), s, recip);
     }
 }
 
@@ -220,11 +231,11 @@ __global__ __launch_bounds__(kThreads) void pagedRead(ReadArgs a) {
 void pagedKvAppendInt8(const PagedCache &c, const void *k, const void *v, const int64_t *slots, size_t rows,
                        llaisysDataType_t dt, int *err, hipStream_t s) {
     if (rows == 0 || c.heads == 0 || c.dim == 0) return;
-    // Few rows: a block of threads each, so that a step of one token per request runs in one round.
-    // Many: 16 rows a block (a cache block has 16 rows or more, so that prompts find one or two beginnings there).
+    // Few rows: a group of threads each, so that a step of one token per request runs in one round.  Many: 16 rows a
+    // group (a cache block has 16 rows or more, so that prompts find one or two beginnings there).
     const int chunk = rows * c.heads * 2 <= 16384 ? 1 : 16;
     const AppendArgs a{{c.k_codes, c.v_codes}, {c.k_scale, c.v_scale}, {k, v}, slots, int64_t(rows),
-                       int64_t(c.n_blocks * c.block), int(c.heads), int(c.dim), __builtin_ctzll(c.block), chunk, err};
+                       int64_t(c.n_blocks * c.block), int(c.heads), int(c.dim), __builtin_ctzll(c.block), chunk, DivU64(c.dim / (dt == LLAISYS_DTYPE_F32 ? 4 : 8)), err};
     const dim3 grid(unsigned((rows + chunk - 1) / chunk), unsigned(c.heads), 2);
     switch (dt) {
     case LLAISYS_DTYPE_F32: pagedAppend<F32><<<grid, kThreads, 0, s>>>(a); return;
