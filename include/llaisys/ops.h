@@ -190,7 +190,8 @@ __C {
      * row_starts[r + 1] - 1; slots and pos_ids [rows] I64: each row's slot and position (for
      * llaisysROPEQK), -1 and 0 behind the last row.  A step that asks for more rows than slots holds,
      * more blocks than are free, a length below 0 or beyond width * block, or with a state that is
-     * none, is refused as a whole: error 2, no rows, table, ring and state as they were. */
+     * none, is refused as a whole: error 2, no rows, table, ring and state as they were.  At most 8192
+     * requests. */
     __export void llaisysPagedTables(llaisysTensor_t block_table, llaisysTensor_t slots,
                                      llaisysTensor_t pos_ids, llaisysTensor_t row_starts,
                                      llaisysTensor_t free_out, llaisysTensor_t old_lens,

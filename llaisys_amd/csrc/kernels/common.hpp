@@ -17,6 +17,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace llaisys::kernels {
 
@@ -242,6 +243,20 @@ __device__ __forceinline__ V groupReduce(V v, V *red) {
         ldsBarrier();
     }
     return v;
+}
+
+// Inclusive sums over the wave's lanes, without LDS: shifts within rows of 16 lanes, then of the rows' last lanes.
+__device__ __forceinline__ unsigned waveScan(unsigned v) {
+    const auto add = [](unsigned x, auto ctrl, auto rows, auto banks) {
+        return x + unsigned(__builtin_amdgcn_update_dpp(0, int(x), decltype(ctrl)::value, decltype(rows)::value, decltype(banks)::value, false));
+    };
+    using std::integral_constant;
+    v = add(v, integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{}, integral_constant<int, 0xF>{}); // row_shr:1
+    v = add(v, integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{}, integral_constant<int, 0xF>{}); // row_shr:2
+    v = add(v, integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{}, integral_constant<int, 0xE>{}); // row_shr:4
+    v = add(v, integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{}, integral_constant<int, 0xC>{}); // row_shr:8
+    v = add(v, integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{}, integral_constant<int, 0xF>{}); // row_bcast:15
+    return add(v, integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{}, integral_constant<int, 0xF>{}); // row_bcast:31
 }
 
 // swiglu of one element, reference src/ops/swiglu/cpu/swiglu_cpu.cpp:15-20: u * (g / (1 +

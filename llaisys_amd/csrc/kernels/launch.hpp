@@ -199,8 +199,8 @@ struct PagedTablesCall {
     size_t requests, width, rows, ring_size, block;
     int *err;
 };
-// Scratch that pagedTables needs for these sizes.
-size_t pagedTablesWorkspaceBytes(const PagedTablesCall &c);
+// At most kPagedTablesRequests requests, rows and ring entries below 2^30; `ws`: the library scratch.
+constexpr size_t kPagedTablesRequests = 8192;
 void pagedTables(const PagedTablesCall &c, void *ws, hipStream_t stream);
 
 // Rows k, v [rows, heads, dim] quantized into the slots; a row of negative slot is skipped.

@@ -165,20 +165,6 @@ __device__ __forceinline__ int rowExponent(float top) { return top > 0.0f ? 15 -
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// Inclusive sums over the wave's lanes, without LDS: shifts within rows of 16 lanes, then of the rows' last lanes.
-__device__ __forceinline__ unsigned waveScan(unsigned v) {
-    const auto add = [](unsigned x, auto ctrl, auto rows, auto banks) {
-        return x + unsigned(__builtin_amdgcn_update_dpp(0, int(x), decltype(ctrl)::value, decltype(rows)::value, decltype(banks)::value, false));
-    };
-    using std::integral_constant;
-    v = add(v, integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{}, integral_constant<int, 0xF>{}); // row_shr:1
-    v = add(v, integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{}, integral_constant<int, 0xF>{}); // row_shr:2
-    v = add(v, integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{}, integral_constant<int, 0xE>{}); // row_shr:4
-    v = add(v, integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{}, integral_constant<int, 0xC>{}); // row_shr:8
-    v = add(v, integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{}, integral_constant<int, 0xF>{}); // row_bcast:15
-    return add(v, integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{}, integral_constant<int, 0xF>{}); // row_bcast:31
-}
-
 // What a block of threads works at: a tile of one request's rows and a chunk of its keys.
 struct Item {
     bool any;

@@ -2,22 +2,29 @@
 //
 // With nb(x) = ceil(x / block), request r going from old to new tokens takes blocks nb(old) ..
 // nb(new) - 1 of its table row from a ring of free block ids when it grows, and gives blocks nb(new) ..
-// nb(old) - 1 back when it shrinks.  Both are exclusive sums over the requests: the i-th block taken is
-// ring[(head + i) % F], the i-th given back goes to ring[(tail + i) % F].  Row t of the step (request r,
+// nb(old) - 1 back when it shrinks.  Both are exclusive sums over the requests: the i-th block given back goes
+// to ring[(tail + i) % F], the i-th taken is ring[(head + i) % F].  Row t of the step (request r,
 // starts[r] <= t < starts[r + 1]) is token pos = old[r] + t - starts[r], in slot
 // table[r][pos / block] * block + pos % block.
 //
-// One block scans the requests (pagedPlan); it refuses the whole step before it writes anything.  A row
-// at offset 0 of a table block is the first of a block just taken, so the rows' threads write the table.
+// Bound by latency.  One launch: every group of threads sums over all requests by itself (their lengths are
+// a few kB), keeps the sums in LDS and writes its share of the rows and of the blocks given back, finding
+// requests by bisection.  A row at offset 0 of a block just taken writes it to the table; nobody else reads that
+// entry.  A block given back and taken in the same step is read where it was, in the table, so no group waits
+// for another; only a state that is updated in place is written by the last group to arrive, when all have read it.  A step
+// that cannot be done is refused by every group alike, before it writes anything.  MI355X, the kernel alone: 3.7 us for 8
+// requests of one new token, 9 us for 512 requests with 100511 rows.
 #include "common.hpp"
 #include "launch.hpp"
-#include "rowplan.hpp"
+
+#include <algorithm>
 
 namespace llaisys::kernels {
 
 namespace {
 
-constexpr int kPlanThreads = 1024;
+constexpr int kRowsPerThread = 4;
+constexpr int64_t kMost = int64_t(1) << 30; // rows and ring entries are below
 
 struct TablesArgs {
     int32_t *table;
@@ -27,146 +34,162 @@ struct TablesArgs {
     const int32_t *old_lens, *new_lens;
     int32_t *ring;
     const int64_t *free_in;
-    int64_t requests, width, rows, ring_size;
+    int64_t width;
+    int requests, rows, ring_size;
     int shift; // log2(block)
-    int64_t *taken; // scratch: [requests] sums of blocks taken, then the head before the step
+    unsigned *arrived; // 0 between launches; null: the state is not updated in place
     int *err;
 };
 
-struct Sums {
-    int64_t rows, more, back;
-};
-
-__device__ __forceinline__ int64_t blocksOf(int64_t n, int shift) { return (n + (int64_t(1) << shift) - 1) >> shift; }
-
-__device__ __forceinline__ Sums sumsOf(const TablesArgs &a, int64_t r, bool &ok) {
-    Sums s{0, 0, 0};
-    if (r >= a.requests) return s;
-    const int64_t o = a.old_lens[r], n = a.new_lens[r], most = a.width << a.shift;
-    ok = ok && o >= 0 && n >= 0 && o <= most && n <= most;
-    const int64_t bo = blocksOf(o, a.shift), bn = blocksOf(n, a.shift);
-    s.rows = n > o ? n - o : 0;
-    s.more = bn > bo ? bn - bo : 0;
-    s.back = bo > bn ? bo - bn : 0;
-    return s;
-}
-
-__device__ __forceinline__ int64_t shflUp(int64_t v, int d) {
-    const int lo = __shfl_up(int(uint32_t(uint64_t(v))), d, kWave), hi = __shfl_up(int(v >> 32), d, kWave);
-    return int64_t((uint64_t(uint32_t(hi)) << 32) | uint32_t(lo));
-}
-
-// Exclusive sums over the block's threads; `total` the sums of all.
-__device__ Sums blockScan(Sums v, Sums &total, Sums *red) {
-    Sums in = v;
-    for (int d = 1; d < kWave; d <<= 1) {
-        const Sums up{shflUp(in.rows, d), shflUp(in.more, d), shflUp(in.back, d)};
-        if (int(threadIdx.x % kWave) >= d) in = Sums{in.rows + up.rows, in.more + up.more, in.back + up.back};
+template <int kThreads, int kRequests>
+__global__ __launch_bounds__(kThreads) void pagedStep(TablesArgs a) {
+    constexpr int kWaves = kThreads / kWave;
+    // exclusive sums over the requests, and the whole sums behind the last
+    __shared__ int rows_to[kRequests + 1], more_to[kRequests + 1], back_to[kRequests + 1];
+    __shared__ unsigned part[2][3][kWaves]; // of the waves, alternating
+    __shared__ float far[3][kWaves];
+    __shared__ int last;
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, block = 1 << a.shift;
+    const auto blocksOf = [&](int64_t n) { return int((n + block - 1) >> a.shift); };
+    const int64_t head = a.free_in[0], tail = a.free_in[1], most = a.width << a.shift, f = a.ring_size;
+    bool ok = head >= 0 && tail >= head && tail - head <= f && tail < (int64_t(1) << 62);
+    unsigned carry[3] = {0, 0, 0};
+    float sum[3] = {0, 0, 0}; // of this thread's requests: tells sums that leave 32 bits
+    for (int r0 = 0, turn = 0; r0 < a.requests; r0 += kThreads, turn ^= 1) {
+        const int r = r0 + tid;
+        unsigned v[3] = {0, 0, 0}, to[3];
+        if (r < a.requests) {
+            const int o = a.old_lens[r], n = a.new_lens[r];
+            ok = ok && o >= 0 && n >= 0 && o <= most && n <= most;
+            const int bo = blocksOf(o), bn = blocksOf(n);
+            v[0] = n > o ? unsigned(n - o) : 0;
+            v[1] = bn > bo ? unsigned(bn - bo) : 0;
+            v[2] = bo > bn ? unsigned(bo - bn) : 0;
+        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            to[k] = waveScan(v[k]);
+            sum[k] += float(v[k]);
+            if (lane == kWave - 1) part[turn][k][wave] = to[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            unsigned before = carry[k];
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const unsigned p = part[turn][k][w];
+                before += w < wave ? p : 0;
+                carry[k] += p;
+            }
+            if (r < a.requests) (k == 0 ? rows_to : k == 1 ? more_to : back_to)[r] = int(before + to[k] - v[k]);
+        }
     }
-    const int wave = threadIdx.x / kWave;
+    if (tid == 0) {
+        rows_to[a.requests] = int(carry[0]);
+        more_to[a.requests] = int(carry[1]);
+        back_to[a.requests] = int(carry[2]);
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        const float s = waveGroupReduce<kWave, SumOp>(sum[k]);
+        if (lane == 0) far[k][wave] = s;
+    }
     __syncthreads();
-    if (threadIdx.x % kWave == kWave - 1) red[wave] = in;
-    __syncthreads();
-    Sums before{0, 0, 0};
-    total = Sums{0, 0, 0};
-    for (int w = 0; w < kPlanThreads / kWave; ++w) {
-        if (w == wave) before = total;
-        total = Sums{total.rows + red[w].rows, total.more + red[w].more, total.back + red[w].back};
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        float s = 0.0f;
+        for (int w = 0; w < kWaves; ++w) s += far[k][w];
+        ok = ok && s < 1.5f * float(kMost); // else more than any step may ask for (the sums are off by far less)
     }
-    return Sums{before.rows + in.rows - v.rows, before.more + in.more - v.more, before.back + in.back - v.back};
-}
-
-__global__ __launch_bounds__(kPlanThreads) void pagedPlan(TablesArgs a) {
-    __shared__ Sums red[kPlanThreads / kWave];
-    const int64_t head = a.free_in[0], tail = a.free_in[1], f = a.ring_size;
-    // the totals first: a step that cannot be done changes nothing
-    bool ok = head >= 0 && tail >= head && tail - head <= f && tail <= INT64_MAX / 2;
-    Sums all{0, 0, 0};
-    for (int64_t r0 = 0; r0 < a.requests; r0 += kPlanThreads) {
-        Sums total;
-        blockScan(sumsOf(a, r0 + threadIdx.x, ok), total, red);
-        all = Sums{all.rows + total.rows, all.more + total.more, all.back + total.back};
-    }
-    ok = ok && all.rows <= a.rows && tail + all.back - head <= f && all.more <= tail - head + all.back;
+    const int64_t all_rows = carry[0], more = carry[1], back = carry[2];
+    ok = ok && all_rows <= a.rows && tail + back - head <= f && more <= tail - head + back;
     ok = __syncthreads_and(ok);
+
+    if (blockIdx.x == 0)
+        for (int r = tid; r <= a.requests; r += kThreads) a.starts[r] = ok ? rows_to[r] : 0;
+    const int first = int(blockIdx.x) * kThreads * kRowsPerThread;
     if (!ok) {
-        for (int64_t r = threadIdx.x; r <= a.requests; r += kPlanThreads) a.starts[r] = 0;
-        if (threadIdx.x == 0) {
+        for (int t = first + tid; t < min(a.rows, first + kThreads * kRowsPerThread); t += kThreads) {
+            a.slots[t] = -1;
+            a.pos[t] = 0;
+        }
+        if (blockIdx.x == 0 && tid == 0) {
             a.free_out[0] = head;
             a.free_out[1] = tail;
             atomicOr(a.err, kErrPagedTables);
         }
         return;
     }
-    Sums carry{0, 0, 0};
-    for (int64_t r0 = 0; r0 < a.requests; r0 += kPlanThreads) {
-        const int64_t r = r0 + threadIdx.x;
-        Sums total;
-        const Sums mine = sumsOf(a, r, ok);
-        Sums at = blockScan(mine, total, red);
-        at = Sums{carry.rows + at.rows, carry.more + at.more, carry.back + at.back};
-        if (r < a.requests) {
-            a.starts[r] = int32_t(at.rows);
-            a.taken[r] = at.more;
+    // the request r of the i-th row, or block: to[r] <= i < to[r + 1]
+    const auto requestOf = [&](const int *to, int i) {
+        int lo = 0, hi = a.requests;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            (to[mid] <= i ? lo : hi) = mid;
         }
-        // blocks given back: a wave copies one request's at a time
-        for (uint64_t left = __ballot(mine.back > 0); left; left &= left - 1) {
-            const int l = __ffsll(static_cast<unsigned long long>(left)) - 1;
-            const int64_t n = __shfl(int(mine.back), l, kWave);
-            const int64_t to = (int64_t(__shfl(int(at.back >> 32), l, kWave)) << 32) |
-                               uint32_t(__shfl(int(uint32_t(at.back)), l, kWave));
-            const int64_t q = r - int64_t(threadIdx.x % kWave) + l;
-            const int64_t first = blocksOf(a.new_lens[q], a.shift);
-            for (int64_t i = threadIdx.x % kWave; i < n; i += kWave)
-                a.ring[(tail + to + i) % f] = a.table[q * a.width + first + i];
+        return lo;
+    };
+    const int ring_head = f ? int(head % f) : 0, ring_tail = f ? int(tail % f) : 0, held = int(tail - head);
+    const auto given = [&](int i) { // the i-th block given back
+        const int r = requestOf(back_to, i);
+        return a.table[r * a.width + blocksOf(a.new_lens[r]) + i - back_to[r]];
+    };
+    const auto inRing = [&](int from, int i) { return int64_t(from) + i < f ? from + i : from + i - a.ring_size; };
+#pragma unroll
+    for (int k = 0; k < kRowsPerThread; ++k) {
+        const int t = first + k * kThreads + tid;
+        if (t >= a.rows) break;
+        int64_t slot = -1, p = 0;
+        if (t < all_rows) {
+            const int r = requestOf(rows_to, t), o = a.old_lens[r];
+            p = int64_t(o) + t - rows_to[r];
+            const int b = int(p >> a.shift), off = int(p) & (block - 1), bo = blocksOf(o);
+            int32_t *entry = a.table + r * a.width + b;
+            int id;
+            if (b < bo) {
+                id = *entry;
+            } else {
+                const int i = more_to[r] + b - bo;
+                id = i < held ? a.ring[inRing(ring_head, i)] : given(i - held);
+                if (off == 0) *entry = id;
+            }
+            if (id < 0) atomicOr(a.err, kErrPagedIndex); // no block: the row is skipped, and said
+            else slot = (int64_t(id) << a.shift) + off;
         }
-        carry = Sums{carry.rows + total.rows, carry.more + total.more, carry.back + total.back};
+        a.slots[t] = slot;
+        a.pos[t] = p;
     }
-    if (threadIdx.x == 0) {
-        a.starts[a.requests] = int32_t(carry.rows);
-        a.taken[a.requests] = head;
-        a.free_out[0] = head + carry.more;
-        a.free_out[1] = tail + carry.back;
-    }
-}
+    for (int64_t i = int64_t(blockIdx.x) * kThreads + tid; i < back; i += int64_t(gridDim.x) * kThreads)
+        a.ring[inRing(ring_tail, int(i))] = given(int(i));
 
-__global__ __launch_bounds__(256) void pagedRows(TablesArgs a) {
-    const int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x;
-    if (t >= a.rows) return;
-    if (t >= a.starts[a.requests]) {
-        a.slots[t] = -1;
-        a.pos[t] = 0;
-        return;
+    if (a.arrived) {
+        if (tid == 0) {
+            const unsigned before = __hip_atomic_fetch_add(a.arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            last = before == gridDim.x - 1;
+            if (last) __hip_atomic_store(a.arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
     }
-    int64_t lo = 0, hi = a.requests; // starts[lo] <= t < starts[hi]
-    while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) / 2;
-        (a.starts[mid] <= t ? lo : hi) = mid;
+    if (tid == 0 && (a.arrived ? last != 0 : blockIdx.x == 0)) {
+        a.free_out[0] = head + more;
+        a.free_out[1] = tail + back;
     }
-    const int64_t o = a.old_lens[lo], p = o + t - a.starts[lo], b = p >> a.shift, off = p & ((int64_t(1) << a.shift) - 1);
-    const int64_t bo = blocksOf(o, a.shift);
-    int32_t id;
-    if (b < bo) {
-        id = a.table[lo * a.width + b];
-    } else {
-        id = a.ring[(a.taken[a.requests] + a.taken[lo] + b - bo) % a.ring_size];
-        if (off == 0) a.table[lo * a.width + b] = id;
-    }
-    if (id < 0) atomicOr(a.err, kErrPagedIndex); // no block: the row is skipped, and said
-    a.slots[t] = id < 0 ? -1 : (int64_t(id) << a.shift) + off;
-    a.pos[t] = p;
 }
 
 } // namespace
 
-size_t pagedTablesWorkspaceBytes(const PagedTablesCall &c) { return (c.requests + 1) * sizeof(int64_t); }
-
 void pagedTables(const PagedTablesCall &c, void *ws, hipStream_t s) {
+    const bool small = c.requests <= 1024;
+    const size_t per_group = (small ? 256 : 1024) * kRowsPerThread;
+    const unsigned groups = unsigned(std::max<size_t>(1, (c.rows + per_group - 1) / per_group));
     const TablesArgs a{c.table, c.slots, c.pos, c.starts, c.free_out, c.old_lens, c.new_lens, c.ring, c.free_in,
-                       int64_t(c.requests), int64_t(c.width), int64_t(c.rows), int64_t(c.ring_size),
-                       __builtin_ctzll(c.block), static_cast<int64_t *>(ws), c.err};
-    pagedPlan<<<1, kPlanThreads, 0, s>>>(a);
-    if (c.rows) pagedRows<<<unsigned((c.rows + 255) / 256), 256, 0, s>>>(a);
+                       int64_t(c.width), int(c.requests), int(c.rows), int(c.ring_size), __builtin_ctzll(c.block),
+                       c.free_out == c.free_in && groups > 1
+                           ? reinterpret_cast<unsigned *>(static_cast<char *>(ws) + kPagedCountersOffset) : nullptr,
+                       c.err};
+    if (small) pagedStep<256, 1024><<<groups, 256, 0, s>>>(a);
+    else pagedStep<1024, kPagedTablesRequests><<<groups, 1024, 0, s>>>(a);
 }
 
 } // namespace llaisys::kernels

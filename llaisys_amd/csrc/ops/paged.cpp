@@ -68,6 +68,13 @@ size_t checkRows(const tensor_t &k, const tensor_t &v, const tensor_t &slots, co
     return rows;
 }
 
+// Bytes of a contiguous tensor.
+struct Range {
+    const std::byte *begin, *end;
+    Range(const tensor_t &t) : begin(t->data()), end(begin + t->numel() * t->elementSize()) {}
+    bool meets(const Range &o) const { return begin < o.end && o.begin < end; }
+};
+
 template <typename P>
 P *ptr(const tensor_t &t) {
     return reinterpret_cast<P *>(t->data());
@@ -91,25 +98,23 @@ void pagedTables(tensor_t block_table, tensor_t slots, tensor_t pos_ids, tensor_
     ASSERT(slots->numel() == pos_ids->numel(), "PagedTables: slots and pos_ids must have the same length");
     ASSERT(free_in->numel() == 2 && free_out->numel() == 2, "PagedTables: the ring's state is (head, tail)");
     requireBlock(block, op);
-    ASSERT(requests < kLimit && width < kLimit && slots->numel() < kLimit, "PagedTables: sizes must be below 2^31");
+    ASSERT(requests <= kernels::kPagedTablesRequests, "PagedTables: at most " << kernels::kPagedTablesRequests << " requests");
+    ASSERT(width < kLimit && slots->numel() < kLimit / 2 && free_blocks->numel() < kLimit / 2,
+           "PagedTables: rows and free_blocks must be below 2^30");
     // each row of what is written is written once, and nothing that is read changes under its readers
-    const tensor_t *written[] = {&block_table, &slots, &pos_ids, &row_starts, &free_blocks, &free_out};
-    const tensor_t *read[] = {&old_lens, &new_lens, &free_in};
-    for (size_t i = 0; i < 6; ++i) {
-        for (size_t j = i + 1; j < 6; ++j)
-            ASSERT(!overlaps(*written[i], *written[j]), "PagedTables: outputs must not overlap");
-        for (const tensor_t *r : read)
-            ASSERT(!overlaps(*written[i], *r) || (written[i] == &free_out && r == &free_in && free_in->data() == free_out->data()),
+    const Range written[] = {block_table, slots, pos_ids, row_starts, free_blocks, free_out}, read[] = {old_lens, new_lens, free_in};
+    for (const Range *w = written; w != written + 6; ++w) {
+        for (const Range *o = w + 1; o != written + 6; ++o) ASSERT(!w->meets(*o), "PagedTables: outputs must not overlap");
+        for (const Range &r : read)
+            ASSERT(!w->meets(r) || (w == written + 5 && &r == read + 2 && r.begin == w->begin),
                    "PagedTables: outputs must not overlap inputs (free_out may be free_in)");
     }
     auto s = streamFor(block_table);
-    kernels::PagedTablesCall c{ptr<int32_t>(block_table), ptr<int64_t>(slots), ptr<int64_t>(pos_ids), ptr<int32_t>(row_starts),
+    const kernels::PagedTablesCall c{ptr<int32_t>(block_table), ptr<int64_t>(slots), ptr<int64_t>(pos_ids), ptr<int32_t>(row_starts),
                                ptr<int64_t>(free_out), ptr<const int32_t>(old_lens), ptr<const int32_t>(new_lens),
                                ptr<int32_t>(free_blocks), ptr<const int64_t>(free_in), requests, width, slots->numel(),
                                free_blocks->numel(), block, device::amd::errorWord(block_table->deviceId())};
-    char *ws = static_cast<char *>(device::amd::workspace(block_table->deviceId(),
-                                                          kernels::kScratchReserved + kernels::pagedTablesWorkspaceBytes(c)));
-    kernels::pagedTables(c, ws + kernels::kScratchReserved, s);
+    kernels::pagedTables(c, device::amd::workspace(block_table->deviceId(), kernels::kScratchReserved), s);
     launched("pagedTables");
 }
 

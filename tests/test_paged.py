@@ -54,6 +54,7 @@ TABLES = CACHE + "tab, st, ln, l2, ring, fi, fo, sl, po = t((2,2), I32), t((3,),
     (TABLES.format("tab, sl, sl, st, fo, ln, l2, ring, fi, 16"), "outputs must not overlap"),
     (TABLES.format("tab, sl, po, st, fo, ln, l2, tab.view(4), fi, 16"), "outputs must not overlap"),
     (TABLES.format("tab, sl, po, st, fo, tab.view(4).slice(0,0,2), l2, ring, fi, 16"), "must not overlap inputs"),
+    (TABLES.format("t((8193,1), I32), sl, po, t((8194,), I32), fo, t((8193,), I32), t((8193,), I32), ring, fi, 16"), "at most 8192 requests"),
     (TABLES.format("tab, sl, po, st, t((3,), I64), ln, l2, ring, fi, 16"), "the ring's state is (head, tail)"),
 ])
 def test_refusals(code, message):

@@ -91,6 +91,10 @@ def test_tables_edges():
     Tables([33, 0, 5], [0, 48, 5], 16, 48, ring=0, spare=0).check(in_place=True)  # blocks given back are taken in the same step
     Tables([100, 7, 64], [0, 0, 0], 16, 3, ring=2).check()  # all end
     Tables([0], [70000], 16, 70000, head=10 ** 12).check()  # one long prompt, a ring that has turned many times
+    # many groups of threads, a state updated in place, blocks given back and taken in the same step
+    Tables([12000, 5, 0, 700, 64], [0, 4000, 8000, 1, 70], 16, 13000, head=77, ring=0, spare=0).check(in_place=True)
+    Tables([9000, 5, 0, 700, 64], [0, 4000, 8000, 1, 70], 16, 13000, head=77, spare=9).check()
+    Tables(_lens(8192, 30, 5), _lens(8192, 60, 6), 16, 200000, head=5).check(in_place=True)
 
 
 def test_tables_refuse_what_cannot_be_done():
