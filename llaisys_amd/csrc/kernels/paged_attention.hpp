@@ -18,6 +18,7 @@
 #include "common.hpp"
 #include "launch.hpp"
 #include "quantize.hpp"
+#include "rowplan.hpp"
 
 #include <type_traits>
 
@@ -32,20 +33,6 @@ constexpr int kLeast = 4;          // steps of a chunk: a multiple of this
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kCodeUnit = 0x1p-9f; // a code's f16 value is code * kCodeUnit
 constexpr float kWeightBits = 15.0f; // weights are 2^(t - m + kWeightBits)
-
-// Division of n < 2^31 by a launch constant d < 2^16.  With 2^s < d <= 2^(s + 1) and m = ceil(2^(32 + s) / d) < 2^32,
-// n m / 2^(32 + s) is above n / d by n (m d - 2^(32 + s)) / (d 2^(32 + s)) < 2^31 2^(s + 1) / (d 2^(32 + s)) = 1 / d, so its
-// whole part is that of n / d.
-struct SmallDiv {
-    uint32_t m = 0, s = 0; // m 0: d is 1
-    SmallDiv() = default;
-    explicit SmallDiv(uint32_t d) {
-        if (d <= 1) return;
-        while ((2u << s) < d) ++s;
-        m = uint32_t(((uint64_t(1) << (32 + s)) + d - 1) / d);
-    }
-    __device__ __forceinline__ int div(int n) const { return m ? int(__umulhi(uint32_t(n), m) >> s) : n; }
-};
 
 struct PagedAttnArgs {
     void *out;

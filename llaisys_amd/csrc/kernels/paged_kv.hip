@@ -9,23 +9,27 @@
 //
 // Quotients are rounded as the exact quotient rounds (ties to even), so that one definition holds for any
 // way of computing it: with n the whole number next to x * (1 / s), off by at most one, e = fma(-n, s, x) is
-// exact (x and n * s agree in all but the last bits), and n is right wherever |e| < s / 2.  Elsewhere (ties, quotients next
-// to one, NaN), and for scales below 2^-96, where 1 / s or e may leave the normal range, the quotient is taken in f64, which
-// tells any two of them from a half apart; so are the older codes.
+// exact (x and n * s agree in all but the last bits), and n is right wherever |e| < s / 2; else (1 in 10^5) it moves by
+// one, or is a tie.  Scales below 2^-96, where 1 / s or e may leave the normal range, divide in f64, which tells any
+// quotient from a half.
 //
 // A group of 256 threads takes `chunk` rows of one head of k or v.  Its slots come in one load of 64, in which every
 // wave finds the rows where cache blocks begin and how far they go; rows stay in registers between the maximum and
-// the codes.  [7598 x 8 heads x 128] bf16, k and v (47 MB): CHUNK_US us.
+// the codes.  The heads of a chunk, k and v, are next to each other in the grid: they read whole rows of the memory then
+// (one head's pieces, a row's length apart, lie in few of its channels).  [7598 x 8 heads x 128] bf16, k and v (47 MB): CHUNK_US us.
 #include "common.hpp"
 #include "launch.hpp"
 #include "quantize.hpp"
 #include "rowplan.hpp"
+
+#include <algorithm>
 
 namespace llaisys::kernels {
 
 namespace {
 
 constexpr int kThreads = 256;
+constexpr size_t kChunksY = 32768;
 
 struct AppendArgs {
     int8_t *codes[2];
@@ -34,7 +38,7 @@ struct AppendArgs {
     const int64_t *slots;
     int64_t rows, slot_end;
     int heads, dim, shift, chunk;
-    DivU64 by_vectors; // of a row
+    SmallDiv by_vectors; // of a row
     int *err;
 };
 
@@ -45,14 +49,14 @@ __device__ __forceinline__ uint32_t codeExact(double x, double s) {
     return uint32_t(int32_t(n)) & 0xFFu;
 }
 
-// Codes of one 16-byte vector; s is the block's scale, recip 1 / s, or NaN where the f32 rule does not hold.
+// Codes of one 16-byte vector; s is the block's scale, recip 1 / s.
 template <typename T>
 __device__ __forceinline__ void storeVec(int8_t *to, const v4u &r, float s, float recip) {
     constexpr int N = Fmt<T>::kVec;
     constexpr float kWhole = 12582912.0f; // 1.5 * 2^23: a sum with it rounds to a whole number, in its low bits
     float f[N];
     Fmt<T>::unpack(r, f);
-    uint32_t c[N];
+    uint32_t c[N], w[N / 4];
     const float half = 0.5f * s;
     bool near = true;
 #pragma unroll
@@ -63,23 +67,62 @@ __device__ __forceinline__ void storeVec(int8_t *to, const v4u &r, float s, floa
     }
     if (__builtin_expect(!near, 0)) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) c[e] = codeExact(f[e], s);
+        for (int e = 0; e < N; ++e) {
+            const float m = __builtin_fmaf(f[e], recip, kWhole), rest = __builtin_fmaf(kWhole - m, s, f[e]);
+            const bool odd = (c[e] & 1u) != 0;
+            c[e] += rest > half || (rest == half && odd) ? 1u : 0u;
+            c[e] -= rest < -half || (rest == -half && odd) ? 1u : 0u;
+            c[e] = f[e] == f[e] ? c[e] : 0u; // NaN
+        }
     }
-    uint32_t w[N / 4];
 #pragma unroll
     for (int e = 0; e < N / 4; ++e) w[e] = packCodes4(c + 4 * e);
     __builtin_memcpy(__builtin_assume_aligned(to, N), w, N);
 }
 
+// Sixteen older codes at s0 as codes at s (in the range of the f32 rule).  c * (s0 / s) in f32 is off by less than 2^-15: only
+// next to a half is it not enough, and c * s0, as a product and its rest, tells there: differences of values that are nearly
+// equal are exact.
+__device__ __forceinline__ void rescale16(int8_t *codes, float s0, float s, float ratio) {
+    const v4u r = *reinterpret_cast<const v4u *>(codes);
+    const uint32_t old[4] = {r.x, r.y, r.z, r.w};
+    uint32_t w[4];
+    const float half = 0.5f * s;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        uint32_t c[4];
+        bool near = true;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const float t = float(int32_t(old[e] << (24 - 8 * b)) >> 24) * ratio, n = rintf(t);
+            near = near && fabsf(t - n) < 0.49996f;
+            c[b] = uint32_t(int32_t(n));
+        }
+        if (__builtin_expect(!near, 0)) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const float x = float(int32_t(old[e] << (24 - 8 * b)) >> 24), p = x * s0, more = __builtin_fmaf(x, s0, -p);
+                const float rest = __builtin_fmaf(-float(int32_t(c[b])), s, p);
+                const float up = (rest - half) + more, down = (rest + half) + more;
+                const bool odd = (c[b] & 1u) != 0;
+                c[b] += up > 0.0f || (up == 0.0f && odd) ? 1u : 0u;
+                c[b] -= down < 0.0f || (down == 0.0f && odd) ? 1u : 0u;
+            }
+        }
+        w[e] = packCodes4(c);
+    }
+    *reinterpret_cast<v4u *>(codes) = v4u{w[0], w[1], w[2], w[3]};
+}
+
 template <typename T>
-__global__ __launch_bounds__(kThreads) void pagedAppend(AppendArgs a) {
+__global__ __launch_bounds__(kThreads, 4) void pagedAppend(AppendArgs a) {
     constexpr int N = Fmt<T>::kVec;
-    constexpr int kKeep = 8; // vectors a thread keeps between the maximum and the codes
+    constexpr int kKeep = 4; // vectors a thread keeps between the maximum and the codes
     __shared__ float red[kThreads / kWave];
-    const int head = blockIdx.y, kv = blockIdx.z, lane = threadIdx.x % kWave;
+    const int head = blockIdx.x / 2, kv = blockIdx.x % 2, lane = threadIdx.x % kWave;
     const int nv = a.dim / N, block = 1 << a.shift;
     // slots t0 - 1 .. t0 + 62; the rows of lanes 1 .. chunk are this group's
-    const int64_t t0 = int64_t(blockIdx.x) * a.chunk;
+    const int64_t t0 = (int64_t(blockIdx.z) * kChunksY + blockIdx.y) * a.chunk;
     const auto slotAt = [&](int64_t t) { return t >= 0 && t < a.rows ? a.slots[t] : int64_t(-1); };
     const int64_t mine = slotAt(t0 - 1 + lane);
     const bool ours = lane >= 1 && lane <= a.chunk;
@@ -115,10 +158,12 @@ __global__ __launch_bounds__(kThreads) void pagedAppend(AppendArgs a) {
             continue;
         }
         const int n = run * nv;
-        const char *in = static_cast<const char *>(a.in[kv]);
+        const size_t from = (size_t(t) * a.heads + head) * a.dim;
+        const char *in = static_cast<const char *>(a.in[kv]) + from * Fmt<T>::kBytes;
+        const unsigned row_elems = unsigned(a.heads) * unsigned(a.dim);
         const auto at = [&](int j) {
-            const int row = int(a.by_vectors.div(uint64_t(j)));
-            return (size_t(t + row) * a.heads + head) * a.dim + size_t(j - row * nv) * N;
+            const int row = a.by_vectors.div(j);
+            return size_t(unsigned(row)) * row_elems + unsigned(j - row * nv) * N;
         };
         const size_t tile = size_t(id) * a.heads + head;
         const float s0 = first ? a.scale[kv][tile] : 0.0f;
@@ -147,29 +192,35 @@ __global__ __launch_bounds__(kThreads) void pagedAppend(AppendArgs a) {
         const float grown = amax / 127.0f, s = grown > s0 ? grown : s0;
         int8_t *codes = a.codes[kv] + (tile << a.shift) * a.dim;
         if (threadIdx.x == 0 && (s != s0 || first == 0)) a.scale[kv][tile] = s;
+        const bool in_f32 = s >= 0x1p-96f && s <= 0x1p120f;
         if (first && s != s0) {
-            for (int j = threadIdx.x; j < first * (a.dim / 16); j += kThreads) {
-                const v4u r = *reinterpret_cast<const v4u *>(codes + j * 16);
-                uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    uint32_t c[4];
-#pragma unroll
-                    for (int b = 0; b < 4; ++b)
-                        c[b] = codeExact(double(int32_t(w[e] << (24 - 8 * b)) >> 24) * double(s0), double(s));
-                    w[e] = packCodes4(c);
-                }
-                *reinterpret_cast<v4u *>(codes + j * 16) = v4u{w[0], w[1], w[2], w[3]};
+            if (__builtin_expect(in_f32, 1)) {
+                const float ratio = s0 / s;
+                for (int j = threadIdx.x; j < first * (a.dim / 16); j += kThreads) rescale16(codes + j * 16, s0, s, ratio);
+            } else {
+#pragma unroll 1
+                for (int j = threadIdx.x; j < first * a.dim; j += kThreads)
+                    codes[j] = int8_t(codeExact(double(codes[j]) * double(s0), double(s)));
             }
         }
-        const float recip = s >= 0x1p-96f && s <= 0x1p120f ? 1.0f / s : __builtin_nanf("");
+        int8_t *const to = codes + first * a.dim;
+        if (__builtin_expect(in_f32, 1)) {
+            const float recip = 1.0f / s;
 #pragma unroll
-        for (int i = 0; i < kKeep; ++i) {
-            const int j = threadIdx.x + i * kThreads;
-            if (j < n) storeVec<T>(codes + first * a.dim + j * N, keep[i], s, recip);
+            for (int i = 0; i < kKeep; ++i) {
+                const int j = threadIdx.x + i * kThreads;
+                if (j < n) storeVec<T>(to + j * N, keep[i], s, recip);
+                __builtin_amdgcn_sched_barrier(0); // one vector's values in registers at a time
+            }
+            for (int j = threadIdx.x + kKeep * kThreads; j < n; j += kThreads)
+                storeVec<T>(to + j * N, load16<T>(in, at(j)), s, recip);
+        } else {
+            for (int j = threadIdx.x; j < n; j += kThreads) {
+                const size_t first_elem = at(j);
+#pragma unroll 1
+                for (int e = 0; e < N; ++e) to[j * N + e] = int8_t(codeExact(double(Fmt<T>::get(in, first_elem + e)), double(s)));
+            }
         }
-        for (int j = threadIdx.x + kKeep * kThreads; j < n; j += kThreads)
-            storeVec<T>(codes + first * a.dim + j * N, load16<T>(in, at(j)), s, recip);
     }
 }
 
@@ -231,12 +282,13 @@ __global__ __launch_bounds__(kThreads) void pagedRead(ReadArgs a) {
 void pagedKvAppendInt8(const PagedCache &c, const void *k, const void *v, const int64_t *slots, size_t rows,
                        llaisysDataType_t dt, int *err, hipStream_t s) {
     if (rows == 0 || c.heads == 0 || c.dim == 0) return;
-    // Few rows: a group of threads each, so that a step of one token per request runs in one round.  Many: 16 rows a
-    // group (a cache block has 16 rows or more, so that prompts find one or two beginnings there).
-    const int chunk = rows * c.heads * 2 <= 16384 ? 1 : 16;
+    // Few rows: a group of threads each, so that a step of one token per request runs in one round.  Many: up to 32 rows
+    // a group (of a prompt, one or two cache blocks begin there).
+    const int chunk = rows * c.heads * 2 <= 16384 ? 1 : int(c.block < 32 ? c.block : 32);
     const AppendArgs a{{c.k_codes, c.v_codes}, {c.k_scale, c.v_scale}, {k, v}, slots, int64_t(rows),
-                       int64_t(c.n_blocks * c.block), int(c.heads), int(c.dim), __builtin_ctzll(c.block), chunk, DivU64(c.dim / (dt == LLAISYS_DTYPE_F32 ? 4 : 8)), err};
-    const dim3 grid(unsigned((rows + chunk - 1) / chunk), unsigned(c.heads), 2);
+                       int64_t(c.n_blocks * c.block), int(c.heads), int(c.dim), __builtin_ctzll(c.block), chunk, SmallDiv(uint32_t(c.dim / (dt == LLAISYS_DTYPE_F32 ? 4 : 8))), err};
+    const size_t chunks = (rows + chunk - 1) / chunk;
+    const dim3 grid(unsigned(2 * c.heads), unsigned(std::min(chunks, kChunksY)), unsigned((chunks + kChunksY - 1) / kChunksY));
     switch (dt) {
     case LLAISYS_DTYPE_F32: pagedAppend<F32><<<grid, kThreads, 0, s>>>(a); return;
     case LLAISYS_DTYPE_BF16: pagedAppend<BF16><<<grid, kThreads, 0, s>>>(a); return;

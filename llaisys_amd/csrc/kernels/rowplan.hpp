@@ -88,6 +88,20 @@ struct DivU64 {
     __device__ uint64_t div(uint64_t i) const { return m == 0 ? i : __umul64hi(i, m); }
 };
 
+// Division of n < 2^31 by a launch constant d < 2^16.  With 2^s < d <= 2^(s + 1) and m = ceil(2^(32 + s) / d) < 2^32,
+// n m / 2^(32 + s) is above n / d by n (m d - 2^(32 + s)) / (d 2^(32 + s)) < 2^31 2^(s + 1) / (d 2^(32 + s)) = 1 / d, so its
+// whole part is that of n / d.
+struct SmallDiv {
+    uint32_t m = 0, s = 0; // m 0: d is 1
+    SmallDiv() = default;
+    explicit SmallDiv(uint32_t d) {
+        if (d <= 1) return;
+        while ((2u << s) < d) ++s;
+        m = uint32_t(((uint64_t(1) << (32 + s)) + d - 1) / d);
+    }
+    __device__ __forceinline__ int div(int n) const { return m ? int(__umulhi(uint32_t(n), m) >> s) : n; }
+};
+
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 inline unsigned blocksFor(size_t work, size_t per_block) {

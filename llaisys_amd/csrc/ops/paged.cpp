@@ -62,7 +62,7 @@ size_t checkRows(const tensor_t &k, const tensor_t &v, const tensor_t &slots, co
     ASSERT(k->shape()[1] == c.heads && k->shape()[2] == c.dim, op << ": kv head shape mismatch");
     const size_t rows = k->shape()[0];
     ASSERT(slots->numel() == rows, op << ": one slot per row");
-    ASSERT(rows < kLimit, op << ": fewer than 2^31 rows");
+    ASSERT(rows < kLimit && rows * c.heads / 8 < size_t(1) << 24, op << ": too many rows and heads for one call");
     requireAligned(k, op);
     requireAligned(v, op);
     return rows;

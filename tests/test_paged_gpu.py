@@ -499,3 +499,18 @@ def test_two_graphs_and_eager_calls_share_the_scratch():
         graphs[1].launch()
         assert np.array_equal(c.run()[1], want[2])
         assert np.array_equal(a.out.numpy(), want[0]) and np.array_equal(b.out.numpy(), want[1])
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_append_rounds_older_codes_as_exact_quotients(dt):
+    # every code at many ratios of scales, ratios of small whole numbers (ties) and others next to them among them
+    rng = np.random.default_rng(8)
+    heads, dim, block, n = 8, 256, 16, 64
+    cache = Cache(n, heads, block, dim)
+    cache.k[:, :, :] = (np.arange(dim) - 128).clip(-127, 127).astype(np.int8)
+    ratio = rng.choice([2.0, 4.0, 6.0, 1.5, 3.0, 10.0, 1.0 + 2.0 ** -20, 1.25, 254.0], (n, heads)) * rng.choice([1.0, 1 + 2.0 ** -23, 1 - 2.0 ** -23], (n, heads))
+    cache.ks = (2.0 ** rng.integers(-20, 20, (n, heads)) * rng.choice([1.0, 1.1, 1.7], (n, heads))).astype(np.float32)
+    k = np.zeros((n, heads, dim))
+    k[:, :, 0] = 127.0 * cache.ks * ratio
+    slots = (np.arange(n) * block + 15).astype(np.int64)
+    _check_append(cache, host(k, dt), host(k, dt), slots, dt)
