@@ -26,10 +26,10 @@ Plan planOf(const PagedAttentionCall &c, size_t tile, size_t most_tiles) {
     const size_t tiles = std::min(rows / tile + requests, most_tiles);
     const size_t steps = (c.width * c.cache.block + kStep - 1) / kStep;
     Plan p{tiles, 0, 0};
-    const size_t per_head = (kTarget + h - 1) / h;
+    const size_t per_head = (kTarget + kTarget / 32 + h - 1) / h + 1;
     if (2 * per_head * h <= kPagedCounters && steps > kLeast) {
-        // the chunks of all tiles are at most the tiles and all steps over a chunk's; those of split tiles at most
-        // twice the latter
+        // the chunks of all tiles are at most the tiles and all steps over a chunk's, which are kTarget over the heads (3%
+        // more, as the sum is rounded); those of split tiles at most twice the latter
         p.target = kTarget;
         p.items = std::min(tiles + per_head, tiles * ((steps + kLeast - 1) / kLeast));
         p.splits = 2 * per_head * h;

@@ -29,7 +29,7 @@ constexpr int kFan = 16;           // chunks merged at once
 constexpr int kPagedThreads = 256; // of a block
 constexpr int kFewTile = 16, kManyTile = 128;
 constexpr int kFewMost = 32;       // rows of a request that go by 16, next to others that do not
-constexpr int kLeast = 4;          // steps of a chunk: a multiple of this
+constexpr int kLeast = 4;          // steps of a chunk, at least
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kCodeUnit = 0x1p-9f; // a code's f16 value is code * kCodeUnit
 constexpr float kWeightBits = 15.0f; // weights are 2^(t - m + kWeightBits)
@@ -193,20 +193,20 @@ __device__ __forceinline__ Item findItem(const PagedAttnArgs &a, int index, bool
     Request q, first;
     bool fine = request(lane, first);
     if (a.target || report) {
-        // (in f32: the sum decides how far keys are split, and is rounded up by more than it can be off)
+        // (in f32: off by less than the 3% that the launch has room for)
         float total = float(tilesOf(first)) * float(stepsOf(first));
         for (int64_t r0 = kWave; r0 < a.requests; r0 += kWave) {
             fine = request(r0 + lane, q) && fine;
             total += float(tilesOf(q)) * float(stepsOf(q));
         }
-        total = waveGroupReduce<kWave, SumOp>(total) * 1.02f;
+        total = waveGroupReduce<kWave, SumOp>(total);
         fine = !__any(!fine);
         if (report && !fine && lane == 0) atomicOr(a.err, kErrPagedIndex);
         // row starts that go back may make more items than the grid has: a tile whose chunks did not all run
         // would leave its counter behind, so nothing is split then
         if (a.target && fine) {
-            const float want = total * float(a.heads) * a.per_target;
-            per = want < 0x1p30f ? (unsigned(want) / kLeast + 1) * kLeast : kAll;
+            const float want = ceilf(total * float(a.heads) * a.per_target);
+            per = want < 0x1p30f ? max(unsigned(want), unsigned(kLeast)) : kAll;
         }
     }
     per = unsigned(uniform(int(per)));
@@ -258,18 +258,24 @@ __device__ __forceinline__ bool cutItem(Item &it, int steps) {
 // ---- partials: [rows of a tile][dim + 4] f32 ---------------------------------------------------
 // 8 channels at a time; behind them a row's maximum and sum, those of the chunk and those of the group of chunks whose
 // merge lies where its first chunk was (each thread overwrites the channels that it alone read).
-// They pass between compute units of different L2s, so they are written and read as device-scope atomics,
-// 8 bytes each, which need no write-back of an L2; a counter of arrivals orders them.
+// They pass between compute units of different L2s, so they are written and read past them (device scope, the
+// sc1 bit), 16 bytes a lane, which needs no write-back or invalidation of an L2; a counter of arrivals orders them.
 
-__device__ __forceinline__ void putPair(float *p, float a, float b) {
-    const uint64_t v = (uint64_t(__float_as_uint(b)) << 32) | __float_as_uint(a);
-    __hip_atomic_store(reinterpret_cast<uint64_t *>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+typedef __amdgpu_buffer_rsrc_t Partials;
+constexpr int kPastL2 = 16; // cache policy: sc1
+
+__device__ __forceinline__ Partials partialsAt(float *p, size_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(p, 0, int(bytes), 0x00020000); // raw, 32-bit elements, bounds in bytes
 }
-__device__ __forceinline__ uint64_t getPair(const float *p) {
-    return __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ __forceinline__ void put4(Partials p, int at, const v4f &v) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, v), p, at * 4, 0, kPastL2);
 }
-__device__ __forceinline__ float firstOf(uint64_t v) { return __uint_as_float(uint32_t(v)); }
-__device__ __forceinline__ float secondOf(uint64_t v) { return __uint_as_float(uint32_t(v >> 32)); }
+__device__ __forceinline__ void put2(Partials p, int at, float a, float b) {
+    __builtin_amdgcn_raw_buffer_store_b64(v2u{__float_as_uint(a), __float_as_uint(b)}, p, at * 4, 0, kPastL2);
+}
+__device__ __forceinline__ v4f get4(Partials p, int at) {
+    return __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(p, at * 4, 0, kPastL2));
+}
 
 // After the whole block's partial stores: true for the block that is the last of `count` to come to the counter.
 __device__ __forceinline__ bool arriveLast(unsigned *counter, unsigned count, unsigned *shared) {
@@ -289,36 +295,32 @@ __device__ __forceinline__ bool arriveLast(unsigned *counter, unsigned count, un
 // Weight of a state of maximum m in a merge of maximum top (a state without keys has -inf).
 __device__ __forceinline__ float mergeWeight(float m, float top) { return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top); }
 
-// Merge of `count` partials, `stride` apart from `first`, in order: calls done(row, c, o, m, l) with 8 channels from c
+// Merge of `count` partials (p's, `stride` floats apart), in order: calls done(row, c, o, m, l) with 8 channels from c
 // on of each valid row, o not yet divided by l.  `level`: of chunks (0), of groups (1).
 template <typename Done>
-__device__ __forceinline__ void mergePartials(const float *first, size_t stride, int count, int level, int dim, int rows, Done &&done) {
+__device__ __forceinline__ void mergePartials(Partials p, int stride, int count, int level, int dim, int rows, Done &&done) {
     const int slots = dim / 8;
     for (int j = threadIdx.x; j < rows * slots; j += kPagedThreads) {
-        const int row = j / slots, c = (j - row * slots) * 8;
-        const float *p = first + size_t(row) * (dim + 4);
+        const int row = j / slots, c = (j - row * slots) * 8, at = row * (dim + 4);
         float m = -INFINITY, l = 0.0f, o[8] = {};
         for (int k0 = 0; k0 < count; k0 += 8) {
-            uint64_t ml[8], x[8][4];
+            v4f ml[8], x[8][2];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 if (k0 + k >= count) continue;
-                const float *pk = p + size_t(k0 + k) * stride;
-                ml[k] = getPair(pk + dim + 2 * level);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[k][e] = getPair(pk + c + 2 * e);
+                const int pk = at + (k0 + k) * stride;
+                ml[k] = get4(p, pk + dim);
+                x[k][0] = get4(p, pk + c);
+                x[k][1] = get4(p, pk + c + 4);
             }
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 if (k0 + k >= count) continue;
-                const float mk = firstOf(ml[k]), top = fmaxf(m, mk);
+                const float mk = level ? ml[k].z : ml[k].x, lk = level ? ml[k].w : ml[k].y, top = fmaxf(m, mk);
                 const float wa = mergeWeight(m, top), wb = mergeWeight(mk, top);
-                l = l * wa + secondOf(ml[k]) * wb;
+                l = l * wa + lk * wb;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    o[2 * e] = o[2 * e] * wa + firstOf(x[k][e]) * wb;
-                    o[2 * e + 1] = o[2 * e + 1] * wa + secondOf(x[k][e]) * wb;
-                }
+                for (int e = 0; e < 8; ++e) o[e] = o[e] * wa + x[k][e / 4][e % 4] * wb;
                 m = top;
             }
         }
@@ -352,32 +354,33 @@ __device__ __forceinline__ void finishItem(const PagedAttnArgs &a, const Item &i
         all(put);
         return;
     }
-    const size_t size = size_t(kTile) * (dim + 4), stride = size * a.heads;
-    float *const base = a.part + (size_t(it.split) * a.heads + head) * size; // of the tile's first chunk
-    const auto keep = [&](int chunk, int level) {
-        float *to = base + size_t(chunk) * stride;
-        return [&, to, level](int row, int c, const float *o, float m, float l) {
-            float *p = to + size_t(row) * (dim + 4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) putPair(p + c + 2 * e, o[2 * e], o[2 * e + 1]);
-            if (c == 0) putPair(p + dim + 2 * level, m, l);
+    const int size = kTile * (dim + 4), stride = size * a.heads;
+    // of the tile's chunks from one of them on, of a group's at the least
+    const auto partials = [&](int chunk, int count) {
+        return partialsAt(a.part + (size_t(it.split + unsigned(chunk)) * a.heads + head) * size, (size_t(count - 1) * stride + size) * sizeof(float));
+    };
+    const auto keep = [&](Partials p, int level) {
+        return [&, p, level](int row, int c, const float *o, float m, float l) {
+            const int at = row * (dim + 4);
+            put4(p, at + c, v4f{o[0], o[1], o[2], o[3]});
+            put4(p, at + c + 4, v4f{o[4], o[5], o[6], o[7]});
+            if (c == 0) put2(p, at + dim + 2 * level, m, l);
         };
     };
-    all(keep(it.chunk, 0));
+    all(keep(partials(it.chunk, 1), 0));
     const auto counter = [&](int level, int chunk) {
         return a.arrived + size_t(level) * kPagedCounters + size_t(it.split + unsigned(chunk)) * a.heads + head;
     };
     const int group0 = it.chunk / kFan * kFan, in_group = min(kFan, it.chunks - group0);
     if (!arriveLast(counter(0, group0), unsigned(in_group), shared)) return;
-    const float *group = base + size_t(group0) * stride;
     if (it.chunks <= kFan) {
-        mergePartials(group, stride, in_group, 0, dim, rows, put);
+        mergePartials(partials(group0, in_group), stride, in_group, 0, dim, rows, put);
         return;
     }
     const int groups = (it.chunks + kFan - 1) / kFan;
-    mergePartials(group, stride, in_group, 0, dim, rows, keep(group0, 1));
+    mergePartials(partials(group0, in_group), stride, in_group, 0, dim, rows, keep(partials(group0, 1), 1));
     if (!arriveLast(counter(1, 0), unsigned(groups), shared)) return;
-    mergePartials(base, stride * kFan, groups, 1, dim, rows, put);
+    mergePartials(partials(0, (groups - 1) * kFan + 1), stride * kFan, groups, 1, dim, rows, put);
 }
 
 template <typename T>
