@@ -273,6 +273,9 @@ __device__ __forceinline__ void put4(Partials p, int at, const v4f &v) {
 __device__ __forceinline__ void put2(Partials p, int at, float a, float b) {
     __builtin_amdgcn_raw_buffer_store_b64(v2u{__float_as_uint(a), __float_as_uint(b)}, p, at * 4, 0, kPastL2);
 }
+__device__ __forceinline__ v2f get2(Partials p, int at) {
+    return __builtin_bit_cast(v2f, __builtin_amdgcn_raw_buffer_load_b64(p, at * 4, 0, kPastL2));
+}
 __device__ __forceinline__ v4f get4(Partials p, int at) {
     return __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(p, at * 4, 0, kPastL2));
 }
@@ -303,20 +306,21 @@ __device__ __forceinline__ void mergePartials(Partials p, int stride, int count,
     for (int j = threadIdx.x; j < rows * slots; j += kPagedThreads) {
         const int row = j / slots, c = (j - row * slots) * 8, at = row * (dim + 4);
         float m = -INFINITY, l = 0.0f, o[8] = {};
-        for (int k0 = 0; k0 < count; k0 += 8) {
-            v4f ml[8], x[8][2];
+        for (int k0 = 0; k0 < count; k0 += kFan) {
+            v2f ml[kFan];
+            v4f x[kFan][2];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
+            for (int k = 0; k < kFan; ++k) {
                 if (k0 + k >= count) continue;
                 const int pk = at + (k0 + k) * stride;
-                ml[k] = get4(p, pk + dim);
+                ml[k] = get2(p, pk + dim + 2 * level);
                 x[k][0] = get4(p, pk + c);
                 x[k][1] = get4(p, pk + c + 4);
             }
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
+            for (int k = 0; k < kFan; ++k) {
                 if (k0 + k >= count) continue;
-                const float mk = level ? ml[k].z : ml[k].x, lk = level ? ml[k].w : ml[k].y, top = fmaxf(m, mk);
+                const float mk = ml[k].x, lk = ml[k].y, top = fmaxf(m, mk);
                 const float wa = mergeWeight(m, top), wb = mergeWeight(mk, top);
                 l = l * wa + lk * wb;
 #pragma unroll
