@@ -13,7 +13,7 @@ namespace llaisys::kernels {
 
 namespace {
 
-constexpr unsigned kTarget = 512; // chunks over all heads: two blocks on each of 256 compute units
+constexpr unsigned kTarget = 512; // chunks over all heads
 
 // What the sizes known to the host allow: the requests' lengths are on the device.
 struct Plan {
@@ -21,10 +21,10 @@ struct Plan {
     size_t splits; // partials
     unsigned target;
 };
+size_t stepsOf(const PagedAttentionCall &c) { return (c.width * c.cache.block + kStep - 1) / kStep; }
 Plan planOf(const PagedAttentionCall &c, size_t tile, size_t most_tiles) {
     const size_t h = c.cache.heads, rows = c.rows * (c.nh / h), requests = std::min(c.rows, c.requests);
-    const size_t tiles = std::min(rows / tile + requests, most_tiles);
-    const size_t steps = (c.width * c.cache.block + kStep - 1) / kStep;
+    const size_t tiles = std::min(rows / tile + requests, most_tiles), steps = stepsOf(c);
     Plan p{tiles, 0, 0};
     const size_t per_head = (kTarget + kTarget / 32 + h - 1) / h + 1;
     if (2 * per_head * h <= kPagedCounters && steps > kLeast) {
@@ -37,28 +37,41 @@ Plan planOf(const PagedAttentionCall &c, size_t tile, size_t most_tiles) {
     return p;
 }
 
-// Tiles of 16 rows for all requests where they have 32 rows or fewer on average (one launch; a longer request
-// among them is 16 rows a tile, which is slower for its own rows alone), else two launches, each request by its rows.
-bool allFew(const PagedAttentionCall &c) { return c.rows * (c.nh / c.cache.heads) <= kFewMost * c.requests; }
-Plan fewPlan(const PagedAttentionCall &c) { return planOf(c, kFewTile, allFew(c) ? SIZE_MAX : kFewMost / kFewTile * c.requests); }
+// Steps up to which a request of any number of rows goes by 16 of them, or -1.
+int fewSteps(const PagedAttentionCall &c) {
+    const size_t work = c.dt == LLAISYS_DTYPE_F32 ? kFewWork<float> : kFewWork<BF16>, steps = work / std::max(c.rows * c.nh, size_t(1));
+    return steps < size_t(kFewSteps) ? -1 : int(std::min(steps, size_t(INT_MAX / kStep)));
+}
+// One launch, 16 rows a tile, where the requests have 32 rows or fewer on average (a longer one among them is then
+// attended so too, which is slower for its own rows alone) or the table holds no more steps than go so.  Else
+// two launches, each request by its rows and steps.
+bool allFew(const PagedAttentionCall &c) {
+    return c.rows * (c.nh / c.cache.heads) <= kFewRows * c.requests || (fewSteps(c) > 0 && stepsOf(c) <= size_t(fewSteps(c)));
+}
+Plan fewPlan(const PagedAttentionCall &c) {
+    return planOf(c, kFewTile, allFew(c) || fewSteps(c) > 0 ? SIZE_MAX : kFewRows / kFewTile * c.requests);
+}
 Plan manyPlan(const PagedAttentionCall &c) { return planOf(c, kManyTile, SIZE_MAX); }
 
 size_t bytesOf(const PagedAttentionCall &c, const Plan &p, size_t tile) { return p.splits * tile * (c.cache.dim + 4) * sizeof(float); }
 
 template <typename T>
 void launch(PagedAttnArgs a, const PagedAttentionCall &c, bool split, hipStream_t s) {
-    const auto with = [&](const Plan &p, int least, int most) {
-        a.target = split ? p.target : 0;
-        a.per_target = 1.0f / float(kTarget);
-        a.few_most = most;
-        a.many_least = least;
-        return a;
-    };
+    a.per_target = 1.0f / float(kTarget);
+    const bool all = allFew(c);
+    a.few_rows = all ? INT_MAX : kFewRows;
+    a.few_steps = fewSteps(c);
+    const bool one = c.requests == 1 && a.few_steps < 0; // (of any number of rows: others may stand behind them)
+    if (!all && one) a.few_rows = 0;
+    if (!all) {
+        const Plan many = manyPlan(c);
+        a.target = split ? many.target : 0;
+        launchPagedMany<T>(a, unsigned(many.items), s);
+        if (one) return;
+    }
     const Plan few = fewPlan(c);
-    if (allFew(c)) return launchPagedFew<T>(with(few, 0, INT_MAX), unsigned(few.items), s);
-    const Plan many = manyPlan(c);
-    launchPagedMany<T>(with(many, c.requests > 1 ? kFewMost + 1 : 0, INT_MAX), unsigned(many.items), s);
-    if (c.requests > 1) launchPagedFew<T>(with(few, 0, kFewMost), unsigned(few.items), s);
+    a.target = split ? few.target : 0;
+    launchPagedFew<T>(a, unsigned(few.items), s);
 }
 
 } // namespace
@@ -75,7 +88,7 @@ void pagedAttentionInt8KV(const PagedAttentionCall &c, void *ws, size_t ws_bytes
     char *head = static_cast<char *>(ws);
     const PagedAttnArgs a{c.out, c.q, c.cache.k_codes, c.cache.v_codes, c.cache.k_scale, c.cache.v_scale, c.table, c.starts, c.lens,
                           reinterpret_cast<float *>(head + kScratchReserved), reinterpret_cast<unsigned *>(head + kPagedCountersOffset),
-                          0, 0.0f, 0, INT_MAX, int64_t(c.rows), int64_t(c.requests), int64_t(c.width),
+                          0, 0.0f, 0, 0, int64_t(c.rows), int64_t(c.requests), int64_t(c.width),
                           int64_t(c.cache.n_blocks), int(c.nh), int(c.cache.heads), int(c.nh / c.cache.heads), int(c.cache.dim),
                           __builtin_ctzll(c.cache.block), SmallDiv(uint32_t(c.cache.heads)), SmallDiv(uint32_t(c.nh / c.cache.heads)), c.scale, c.err};
     switch (c.dt) {

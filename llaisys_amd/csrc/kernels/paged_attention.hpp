@@ -25,11 +25,20 @@
 namespace llaisys::kernels {
 
 constexpr int kStep = 64;          // keys of a step
-constexpr int kFan = 16;           // chunks merged at once
+constexpr int kFan = 16;           // chunks, and groups of them, merged at once
 constexpr int kPagedThreads = 256; // of a block
 constexpr int kFewTile = 16, kManyTile = 128;
-constexpr int kFewMost = 32;       // rows of a request that go by 16, next to others that do not
-constexpr int kLeast = 4;          // steps of a chunk, at least
+// A request goes by 16 rows where it has 32 or fewer, or where rows * q heads of the call times the request's steps are at most
+// kFewWork, and the steps allowed so are kFewSteps or more: 128-row tiles then leave most compute units idle.  In us by 16 and
+// by 128 rows, 32 / 8 heads of 128, bf16: 1 request of 96 rows over 500 keys before them 14 and 23, of 200 over 500 25 and 24,
+// of 512 over 500 33 and 37, over 1500 59 and 48; 4 of 96 over 1500 41 and 47, over 4000 90 and 82.  f32, whose products
+// are two or three in either: 1 of 512 over 1500 66 and 82, over 4000 135 and 129; 4 of 512 over 500 119 and 96.
+constexpr int kFewRows = 32, kFewSteps = 8;
+template <typename T>
+constexpr size_t kFewWork = std::is_same_v<T, float> ? 1 << 19 : 1 << 18;
+constexpr int kLeast = 4;        // steps of a chunk, at least
+constexpr int kMostChunks = 128; // of a tile: what its merge costs grows with them
+static_assert(kMostChunks <= kFan * kFan, "two levels");
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kCodeUnit = 0x1p-9f; // a code's f16 value is code * kCodeUnit
 constexpr float kWeightBits = 15.0f; // weights are 2^(t - m + kWeightBits)
@@ -44,7 +53,7 @@ struct PagedAttnArgs {
     unsigned *arrived;  // [2][kPagedCounters], 0 between launches
     unsigned target;    // chunks wanted over all requests and heads; 0: no tile is split
     float per_target;   // 1 / target
-    int few_most, many_least; // rows of the requests that the launch attends: up to, from
+    int few_rows, few_steps; // a request goes by 16 rows up to so many rows, or steps
     int64_t rows, requests, width, n_blocks;
     int nh, heads, group, dim, shift;
     SmallDiv by_heads, by_group;
@@ -182,8 +191,8 @@ __device__ __forceinline__ Item findItem(const PagedAttnArgs &a, int index, bool
         if (r >= a.requests) return true;
         const int s0 = a.starts[r], s1 = a.starts[r + 1], k = a.lens[r];
         if (s0 < 0 || s1 < s0 || s1 > a.rows || k < 0 || k > (a.width << a.shift)) return false;
-        const int rows = (s1 - s0) * a.group;
-        if (rows <= a.few_most && rows >= a.many_least) q = Request{s0, s1 - s0, k}; // (else another launch's)
+        const bool few = (s1 - s0) * a.group <= a.few_rows || k <= a.few_steps * kStep;
+        if (few == (kTile == kFewTile)) q = Request{s0, s1 - s0, k}; // (else the other launch's)
         return true;
     };
     const auto tilesOf = [&](const Request &q) { return (unsigned(q.n * a.group) + kTile - 1) / kTile; };
@@ -194,18 +203,20 @@ __device__ __forceinline__ Item findItem(const PagedAttnArgs &a, int index, bool
     bool fine = request(lane, first);
     if (a.target || report) {
         // (in f32: off by less than the 3% that the launch has room for)
-        float total = float(tilesOf(first)) * float(stepsOf(first));
+        float total = float(tilesOf(first)) * float(stepsOf(first)), most = tilesOf(first) ? float(stepsOf(first)) : 0.0f;
         for (int64_t r0 = kWave; r0 < a.requests; r0 += kWave) {
             fine = request(r0 + lane, q) && fine;
             total += float(tilesOf(q)) * float(stepsOf(q));
+            most = fmaxf(most, tilesOf(q) ? float(stepsOf(q)) : 0.0f);
         }
         total = waveGroupReduce<kWave, SumOp>(total);
+        most = waveGroupReduce<kWave, MaxOp>(most);
         fine = !__any(!fine);
         if (report && !fine && lane == 0) atomicOr(a.err, kErrPagedIndex);
         // row starts that go back may make more items than the grid has: a tile whose chunks did not all run
         // would leave its counter behind, so nothing is split then
         if (a.target && fine) {
-            const float want = ceilf(total * float(a.heads) * a.per_target);
+            const float want = ceilf(fmaxf(total * float(a.heads) * a.per_target, most * (1.0f / kMostChunks)));
             per = want < 0x1p30f ? max(unsigned(want), unsigned(kLeast)) : kAll;
         }
     }

@@ -59,9 +59,8 @@ struct StepData {
 
 // NT: 64s of channels, rounded up; D: the head size where it is 64 NT, else 0.
 template <typename T, int NT, int D>
-__global__ __launch_bounds__(kPagedThreads, NT <= 2 ? 2 : 1) void pagedFew(PagedAttnArgs a) {
+__global__ __launch_bounds__(kPagedThreads, NT <= 2 ? 3 : 1) void pagedFew(PagedAttnArgs a) {
     constexpr bool kTwoP = !std::is_same_v<T, BF16>;
-    constexpr bool kAhead = NT <= 2; // the next step's codes fit the registers
     constexpr int kRows = kFewTile, CH = 4 * NT, NW = kFewWaves;
     __shared__ struct {
         float m[NW][kRows], l[NW][kRows];
@@ -219,39 +218,13 @@ __global__ __launch_bounds__(kPagedThreads, NT <= 2 ? 2 : 1) void pagedFew(Paged
             if (m16 < rows && c < dim) raw[t][h].load(a.q, row_at + c);
             else raw[t][h].zero();
         }
-    const auto setRows = [&] {
-        q.set(raw);
-        row_scale = __builtin_amdgcn_ldexpf(a.scale * kLog2e, 9 - q.exponent);
-    };
-    if constexpr (kAhead) {
-        StepData<NT> d0, d1;
-        Ids next{0, 0};
-        const auto fetchNext = [&](StepData<NT> &d) { // the step after `step`, where there is one
-            if (step + NW >= end) return;
-            fetch(step + NW, next, d);
-            if (step + 2 * NW < end) next = ids(step + 2 * NW);
-        };
-        if (step < end) {
-            fetch(step, now, d0);
-            if (step + NW < end) next = ids(step + NW);
-        }
-        setRows();
-        for (; step < end; step += NW) {
-            fetchNext(d1);
-            compute(step, d0);
-            step += NW;
-            if (step >= end) break;
-            fetchNext(d0);
-            compute(step, d1);
-        }
-    } else {
-        setRows();
-        for (; step < end; step += NW) {
-            StepData<NT> d;
-            fetch(step, now, d);
-            if (step + NW < end) now = ids(step + NW);
-            compute(step, d);
-        }
+    q.set(raw);
+    row_scale = __builtin_amdgcn_ldexpf(a.scale * kLog2e, 9 - q.exponent);
+    for (; step < end; step += NW) {
+        StepData<NT> d;
+        fetch(step, now, d);
+        if (step + NW < end) now = ids(step + NW);
+        compute(step, d);
     }
 
     // the waves' states: [row][channel], channel CH (4 quarter + i) + k of lane (row, quarter)

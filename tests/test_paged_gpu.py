@@ -304,6 +304,31 @@ def test_attention_long(rows, lens, dt):
     Attend(rows, lens, 12, 2, 128, 64, dt, seed=4).check()
 
 
+# Rows of a call choose the tiles of its requests, unused ones with them: so many that requests of more than 32 rows go by 128.
+def unused(nh):
+    return 70000 // nh
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("nh,heads,dim", HEADS)
+def test_attention_beside_many_unused_rows(nh, heads, dim, dt):
+    Attend([37, 1, 0, 64, 5, 130], [37, 90, 50, 64, 133, 300], nh, heads, dim, 32, dt, pad=unused(nh), seed=nh + 1).check()
+    Attend([3], [50], nh, heads, dim, 16, dt, pad=unused(nh), seed=nh).check()
+
+
+@pytest.mark.parametrize("rows,lens", [([300], [299]), ([300, 2], [0, 1]), ([70, 1, 300, 90], [30, 0, 5000, 90]), ([1], [0]), ([150], [9000])])
+def test_attention_long_beside_many_unused_rows(rows, lens):
+    Attend(rows, lens, 8, 2, 64, 64, "bf16", pad=unused(8), seed=5).check()
+    Attend(rows, lens, 8, 2, 64, 64, "f32", pad=unused(8), seed=5).check()
+
+
+@pytest.mark.parametrize("rows,lens", [([300, 40, 1], [300, 5000, 2000]), ([512], [2500]), ([40, 1, 200], [9000, 30, 200])])
+def test_attention_tiles_by_steps(rows, lens):
+    # of a call's requests with many rows, those of few steps go by 16 rows and the others by 128
+    for dt in ("bf16", "f32"):
+        Attend(rows, lens, 32, 4, 64, 64, dt, pad=1, seed=8).check()
+
+
 def test_attention_many_requests():
     rng = np.random.default_rng(9)
     lens = [int(x) for x in rng.integers(1, 90, 700)]
@@ -321,10 +346,11 @@ def test_attention_sharp_and_flat_scores():
     a.check()
 
 
+@pytest.mark.parametrize("pad", [0, 17500])
 @pytest.mark.parametrize("dt,lo,hi", [("bf16", 1e-30, 1e30), ("f32", 1e-30, 1e30), ("f16", 1e-7, 3e4)])
-def test_attention_scales_far_apart(dt, lo, hi):
+def test_attention_scales_far_apart(dt, lo, hi, pad):
     # rows of q of very different sizes, blocks of values of very different sizes
-    a = Attend([1, 50, 1], [300, 400, 77], 4, 2, 64, 16, dt, seed=2)
+    a = Attend([1, 50, 1], [300, 400, 77], 4, 2, 64, 16, dt, pad=pad, seed=2)
     rng = np.random.default_rng(1)
     q = ref.widen(a.q)
     size = np.where(np.arange(len(q)) % 2, lo, hi)[:, None, None]
@@ -335,9 +361,10 @@ def test_attention_scales_far_apart(dt, lo, hi):
     a.check()
 
 
-def test_attention_non_finite():
+@pytest.mark.parametrize("pad", [0, 17500])
+def test_attention_non_finite(pad):
     # a block of NaN scale reaches only the rows that see it; a row of q with a NaN only itself
-    a = Attend([1, 60, 1], [100, 60, 64], 4, 2, 64, 16, "bf16", seed=6)
+    a = Attend([1, 60, 1], [100, 60, 64], 4, 2, 64, 16, "bf16", pad=pad, seed=6)
     a.cache.vs[a.table[1, 2], 0] = np.nan  # keys 32..47 of request 1, q heads 0 and 1
     a.cache.ks[a.table[1, 3], 1] = np.nan  # keys 48..59, q heads 2 and 3
     a.table[0, 7] = next(b for b in range(len(a.cache.k)) if b not in a.table)
@@ -351,9 +378,25 @@ def test_attention_non_finite():
     assert np.isnan(got[61, 3]).all() and not np.isnan(got[61, :3]).any() and not np.isnan(got[0]).any()
 
 
-def test_attention_skips_bad_blocks():
+@pytest.mark.parametrize("pad", [0, 17500])
+@pytest.mark.parametrize("value", [-1.0, np.inf, -np.inf, np.nan])
+def test_attention_scales_that_are_no_scales(value, pad):
+    # rows that see such a block are NaN, the others as without it
+    for which in ("ks", "vs"):
+        a = Attend([1, 60], [100, 60], 4, 2, 64, 16, "bf16", pad=pad, seed=6)
+        exp, tol = a.expect()
+        getattr(a.cache, which)[a.table[1, 2], 0] = value  # keys 32..47 of request 1, q heads 0 and 1
+        err, got = a.run()
+        got = ref.widen(got[:61])
+        assert err == 0 and np.isnan(got[33:, :2]).all()
+        got[33:, :2], exp[33:, :2] = 0, 0
+        assert (np.abs(got - exp[:61]) <= tol[:61]).all()
+
+
+@pytest.mark.parametrize("pad", [0, 17500])
+def test_attention_skips_bad_blocks(pad):
     # ids outside the pool: their keys are not attended, and the error word says so
-    a = Attend([1, 40], [200, 90], 4, 2, 64, 16, "bf16", seed=7)
+    a = Attend([1, 40], [200, 90], 4, 2, 64, 16, "bf16", pad=pad, seed=7)
     a.table[0, 3], a.table[1, 1], a.table[1, 0] = -1, len(a.cache.k), 2 ** 31 - 1
     a.check(err=4)
 
