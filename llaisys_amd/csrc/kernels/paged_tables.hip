@@ -12,8 +12,8 @@
 // requests by bisection.  A row at offset 0 of a block just taken writes it to the table; nobody else reads that
 // entry.  A block given back and taken in the same step is read where it was, in the table, so no group waits
 // for another; only a state that is updated in place is written by the last group to arrive, when all have read it.  A step
-// that cannot be done is refused by every group alike, before it writes anything.  MI355X, the kernel alone: 3.7 us for 8
-// requests of one new token, 9 us for 512 requests with 100511 rows.
+// that cannot be done is refused by every group alike, before it writes anything.  MI355X, the kernel alone: 3.6 us for 8
+// requests of one new token, 9.4 us for 512 requests with 100511 rows.
 #include "common.hpp"
 #include "launch.hpp"
 

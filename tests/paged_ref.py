@@ -90,8 +90,8 @@ def attend(q, k_codes, k_scale, v_codes, v_scale, table, starts, lens, scale, we
     and q may enter as two f16 parts, 2^-22 relative; the exponent's argument and the exponential add
     4 u (|s| + |max|) + 4 u.  An error e of every exponent moves a weight by e, and the weighted mean by at most 2 e A.  A weight is rounded to
     weight_step (relative), 2 weight_step A with the sum of weights unrounded; sums of n weights in f32 add 2 n u A.  A weight far
-    below the largest, 1, loses more: it enters the product with the values as f16 times 2^12, next to a scale of its values
-    that is within 8 times of the one they are summed in, so half of f16's smallest step is 2^-25 2^-12 8 = 2^-34 of the
+    below the largest, 1, loses more: it enters the product with the values as f16 times 2^11 or more, and the scale of its
+    values is at most the one they are summed in, so half of f16's smallest step is 2^-25 2^-11, below 2^-34 of the
     largest weight times a value, for each of the n keys.  Storing rounds once."""
     q_bits, q = np.asarray(q), widen(q)
     block, heads, dim = k_codes.shape[2], k_codes.shape[1], k_codes.shape[3]
