@@ -216,9 +216,9 @@ __C {
     /* Causal GQA attention of each request over its blocks: q, attn_val [rows, nh, d] of one float
      * type, the rows of request r row_starts[r] .. row_starts[r + 1] - 1 and its kv_lens[r] (I32)
      * cached tokens, these rows' own among them.  Row i of n sees tokens t <= kv_lens - n + i; f32
-     * softmax of (q . k) * scale; a row that sees nothing gives 0, a NaN score NaN.  Keys of a block id outside the pool
-     * are not attended (error 4); a request whose length or row starts are out of range is skipped
-     * (error 4).  Rows of no request are left as they are.  Outputs round to nearest (F16 too).  Any
+     * softmax of (q . k) * scale; a row that sees nothing gives 0, a NaN score NaN.  Keys of a block id
+     * outside the pool are not attended (error 4; a cache without blocks is refused); a request whose
+     * length or row starts are out of range is skipped (error 4).  Rows of no request are left as they are.  Outputs round to nearest (F16 too).  Any
      * mix of prompts, chunks and single tokens goes in one call. */
     __export void llaisysPagedAttentionInt8KV(llaisysTensor_t attn_val, llaisysTensor_t q,
                                               llaisysTensor_t k_cache, llaisysTensor_t k_scale,

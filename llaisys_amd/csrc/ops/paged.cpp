@@ -158,6 +158,7 @@ void pagedAttentionInt8KV(tensor_t attn_val, tensor_t q, tensor_t k_cache, tenso
     CHECK_SAME_SHAPE(attn_val->shape(), q->shape());
     const size_t rows = q->shape()[0], nh = q->shape()[1];
     ASSERT(q->shape()[2] == c.dim, "PagedAttentionInt8KV: head_dim mismatch");
+    ASSERT(c.n_blocks > 0, "PagedAttentionInt8KV: the cache has no blocks"); // (a bad id is read as block 0)
     ASSERT(c.heads > 0 && nh > 0 && nh % c.heads == 0, "nhead must be divisible by kv_head (GQA)");
     ASSERT(block_table->ndim() == 2, "PagedAttentionInt8KV: block_table [requests, width]");
     const size_t requests = block_table->shape()[0], width = block_table->shape()[1];

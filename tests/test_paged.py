@@ -37,6 +37,7 @@ TABLES = CACHE + "tab, st, ln, l2, ring, fi, fo, sl, po = t((2,2), I32), t((3,),
     (ATTEND.format("o, q, kc, ks, vc, vs, tab, st, ln"), "Unsupported device"),
     (ATTEND.format("o, t((3,4,16)), kc, ks, vc, vs, tab, st, ln"), "Shapes mismatch"),
     (ATTEND.format("t((3,4,16)), t((3,4,16)), kc, ks, vc, vs, tab, st, ln"), "head_dim mismatch"),
+    (ATTEND.format("o, q, t((0,2,16,32), I8), t((0,2)), t((0,2,16,32), I8), t((0,2)), tab, st, ln"), "the cache has no blocks"),
     (ATTEND.format("t((3,3,32)), t((3,3,32)), kc, ks, vc, vs, tab, st, ln"), "divisible by kv_head"),
     (ATTEND.format("t((3,4,32), BF), q, kc, ks, vc, vs, tab, st, ln"), "Datatypes mismatch"),
     (ATTEND.format("o, q, kc, ks, vc, vs, t((2,2), I64), st, ln"), "must be INT32"),
