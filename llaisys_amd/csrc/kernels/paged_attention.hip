@@ -24,16 +24,16 @@ struct Plan {
     unsigned target;
 };
 size_t stepsOf(const PagedAttentionCall &c) { return (c.width * c.cache.block + kStep - 1) / kStep; }
-Plan planOf(const PagedAttentionCall &c, size_t tile, size_t most_tiles) {
+Plan planOf(const PagedAttentionCall &c, size_t tile, size_t least, size_t most_tiles) {
     const size_t h = c.cache.heads, rows = c.rows * (c.nh / h), requests = std::min(c.rows, c.requests);
     const size_t tiles = std::min(rows / tile + requests, most_tiles), steps = stepsOf(c);
     Plan p{tiles, 0, 0};
     const size_t per_head = (kTarget + kTarget / 32 + h - 1) / h + 1;
-    if (2 * per_head * h <= kPagedCounters && steps > kLeast) {
+    if (2 * per_head * h <= kPagedCounters && steps > least) {
         // the chunks of all tiles are at most the tiles and all steps over a chunk's, which are kTarget over the heads (3%
         // more, as the sum is rounded); those of split tiles at most twice the latter
         p.target = kTarget;
-        p.items = std::min(tiles + per_head, tiles * ((steps + kLeast - 1) / kLeast));
+        p.items = std::min(tiles + per_head, tiles * ((steps + least - 1) / least));
         p.splits = 2 * per_head * h;
     }
     return p;
@@ -51,9 +51,9 @@ bool allFew(const PagedAttentionCall &c) {
     return c.rows * (c.nh / c.cache.heads) <= kFewRows * c.requests || (fewSteps(c) > 0 && stepsOf(c) <= size_t(fewSteps(c)));
 }
 Plan fewPlan(const PagedAttentionCall &c) {
-    return planOf(c, kFewTile, allFew(c) || fewSteps(c) > 0 ? SIZE_MAX : kFewRows / kFewTile * c.requests);
+    return planOf(c, kFewTile, kFewLeast, allFew(c) || fewSteps(c) > 0 ? SIZE_MAX : kFewRows / kFewTile * c.requests);
 }
-Plan manyPlan(const PagedAttentionCall &c) { return planOf(c, kManyTile, SIZE_MAX); }
+Plan manyPlan(const PagedAttentionCall &c) { return planOf(c, kManyTile, kManyLeast, SIZE_MAX); }
 
 size_t bytesOf(const PagedAttentionCall &c, const Plan &p, size_t tile) { return p.splits * tile * (c.cache.dim + 4) * sizeof(float); }
 

@@ -36,7 +36,9 @@ constexpr int kFewTile = 16, kManyTile = 128;
 constexpr int kFewRows = 32, kFewSteps = 8;
 template <typename T>
 constexpr size_t kFewWork = std::is_same_v<T, float> ? 1 << 19 : 1 << 18;
-constexpr int kLeast = 4;        // steps of a chunk, at least
+// Steps of a chunk, at least: a 128-row tile's partial is 8 times as large (us of 512 rows after some 1000 keys beside 24 single
+// ones: 4 58, 8 52).
+constexpr int kFewLeast = 4, kManyLeast = 8;
 constexpr int kMostChunks = 256; // of a tile, merged on two levels (131072 keys: 256 22.7 us, 128 25.4)
 static_assert(kMostChunks <= kFan * kFan, "two levels");
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -230,7 +232,7 @@ __device__ __forceinline__ Item findItem(const PagedAttnArgs &a, int index, bool
         // would leave its counter behind, so nothing is split then
         if (a.target && fine) {
             const float want = ceilf(fmaxf(total * float(a.heads) * a.per_target, most * (1.0f / kMostChunks)));
-            per = want < 0x1p30f ? max(unsigned(want), unsigned(kLeast)) : kAll;
+            per = want < 0x1p30f ? max(unsigned(want), unsigned(kTile == kFewTile ? kFewLeast : kManyLeast)) : kAll;
         }
     }
     per = unsigned(uniform(int(per)));
@@ -239,8 +241,12 @@ __device__ __forceinline__ Item findItem(const PagedAttnArgs &a, int index, bool
         if (r0) request(r0 + lane, q);
         else q = first;
         const unsigned tiles = tilesOf(q), steps = stepsOf(q);
+        // Chunks of a request have one length.  128-row tiles fill the compute units' places with few blocks, and one too many
+        // is a round more: as many as come next to `per` steps.  us: 64 ragged tokens, 16 rows a tile, rounded up 57.3 (with a
+        // shorter last chunk 61.5), to the nearest 63.9; 2 chunks of 700 rows after 200, 128 a tile, 53.9 and 37.3.
         unsigned chunks = 1;
-        if (__any(steps > per)) chunks = steps > per ? (steps + per - 1) / per : 1;
+        if (__any(steps > per)) chunks = steps > per ? (steps + (kTile == kFewTile ? per - 1 : per / 2)) / per : 1;
+        const unsigned part = chunks > 1 ? (steps + chunks - 1) / chunks : kAll;
         const unsigned mine = tiles * chunks, split = chunks > 1 ? mine : 0;
         const unsigned to = waveScan(mine), sto = __any(chunks > 1) ? waveScan(split) : 0;
         const unsigned at = unsigned(index - items); // before the group where it wraps
@@ -259,8 +265,8 @@ __device__ __forceinline__ Item findItem(const PagedAttnArgs &a, int index, bool
             it.tile = of(tiles) - 1 - t; // the last sees most keys: first
             it.chunk = in - t * c;
             it.chunks = c;
-            it.step0 = it.chunk * int(per);
-            it.step1 = c == 1 ? int(kAll) : it.step0 + int(per);
+            it.step0 = it.chunk == 0 ? 0 : it.chunk * of(part);
+            it.step1 = it.step0 + of(part);
             it.split = unsigned(uniform(splits) + of(sto - split) + t * c);
             return it;
         }

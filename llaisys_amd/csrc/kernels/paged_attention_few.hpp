@@ -5,7 +5,7 @@
 // the scores a lane gets are those of the 16 keys whose values it loads: no exchange between lanes, no LDS
 // until the waves' states merge.  V's codes are transposed by the byte permutes that widen them.
 // Three blocks a compute unit hide each other's loads; a step ahead in registers leaves room for two.  us, bf16,
-// heads of 128: 64 tokens over 100 to 8192 keys each, 32 / 8 heads, 61.6 (3.8 TB/s; two blocks and a step ahead 67.6), one over
+// heads of 128: 64 tokens over 100 to 8192 keys each, 32 / 8 heads, 56.9 (4.1 TB/s; before the chunks had one length 61.6, two blocks and a step ahead 67.6), one over
 // 131072, 12 / 2 heads, 22.7 (3.0 TB/s, the two merges among them; 25.6), one over 200 7.0: latency of the search, of
 // ids, codes and the waves' merge, one behind the other.
 #pragma once

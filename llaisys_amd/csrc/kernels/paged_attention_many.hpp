@@ -8,7 +8,7 @@
 // reads nor the writes meet in a bank.
 //
 // Bound by each wave's chain of LDS reads, products, maximum and weights, of which the registers let two blocks of waves run
-// on a compute unit: 3 prompts, 8419 rows, 32 / 8 heads of 128, bf16, take 256 us (758 TFLOP/s; a large product reaches
+// on a compute unit: 3 prompts, 8419 rows, 32 / 8 heads of 128, bf16, take 253 us (766 TFLOP/s; a large product reaches
 // 1157), and leaving out the exponentials did not change that.
 #pragma once
 
